@@ -13,7 +13,10 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libosp_hip.so")
 OBJDIR = os.path.join(HERE, "csrc", "_obj")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-Wno-unused-result"]
+#: the packed f32 instructions stay off: some of their forms have given wrong results now and then, with no error (scalar and packed
+#: forms round alike, so results do not change; the host pass warns that it does not know the feature, which is harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
