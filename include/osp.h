@@ -277,6 +277,16 @@ int osp_conv2d_dgrad_bf16(const void* dy, int64_t dy_bf16, const void* wt, int64
 /* replaces: same call sites as osp_conv_gemm_f32 (f32 operands in HBM), products as three bf16 MFMAs over (hi, lo) operand pairs: the 'mixed' parity mode's generator GEMMs outside the index-critical path */
 int osp_conv_gemm_f32_split(const float* A, int64_t lda, int64_t M, int64_t T, int64_t Cin, int64_t taps, int64_t pad, const float* a_rowscale, const float* B, int64_t sBn, int64_t sBtap, int64_t sBk, int64_t N, float* C, int64_t ldc, int64_t epi, const float* bias, const float* gamma, const float* res, int64_t ldr, const float* rowmask, const float* rowscale, float* aux_out, const float* aux_in, int64_t ld_aux, int64_t batch, int64_t sAb, int64_t sBb, int64_t sCb, int64_t sXb, int64_t accumulate, hipStream_t stream);
 
+/* ---- group_norm.hip ---- */
+/* replaces: workspace query for osp_group_norm_fwd / osp_group_norm_bwd */
+int64_t osp_group_norm_workspace_bytes(int64_t B, int64_t M, int64_t C, int64_t G, int64_t backward);
+
+/* replaces: no reference counterpart: group norm + activation over the rows of each document (the place of BatchNorm + swish in _conformer/convolution.py:61-70, which counts padded frames) */
+int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, void* y, float* mean, float* rstd, void* workspace, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, float eps, int64_t act, hipStream_t stream);
+
+/* replaces: autograd of the same */
+int osp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, const float* mean, const float* rstd, void* dx, float* dw, float* db, void* workspace, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M, int64_t C, int64_t G, int64_t act, hipStream_t stream);
+
 /* ---- loss.hip ---- */
 /* replaces: FastSpeech2Loss.forward generator/loss.py:83-140, DurationPredictorLoss :28-46 */
 int osp_variance_losses(const float* d_hat, const float* p_hat, const float* e_hat, const float* ds, const float* ps, const float* es, const int64_t* x_len, float clip_val, float* out, float* gd, float* gp, float* ge, int64_t B, int64_t T, hipStream_t stream);
@@ -313,6 +323,17 @@ int osp_sumsq(const float* g, int64_t n, double* out, hipStream_t stream);
 
 /* replaces: torch.optim.AdamW.step + clip_gradients: base_lightning_module.py:96-105,116-125; configs/model/optimizer/adamw.yaml */
 int osp_adamw_clip(float* p, const float* g, float* m, float* v, int64_t n, const double* sumsq, const float* lr_dev, const int64_t* step_dev, float lr, float beta1, float beta2, float eps, float wd, int64_t step, float max_norm, float gscale, hipStream_t stream);
+
+/* ---- packed_rows.hip ---- */
+/* replaces: no reference counterpart: most tiles the tile list of a packed batch can have (the reference pads every batch) */
+int64_t osp_packed_rows_tiles(int64_t B, int64_t M);
+
+/* replaces: no reference counterpart: documents and tile list of a packed or padded batch, from offsets / lengths on the device */
+int osp_packed_rows_plan(const int64_t* src, int64_t padded, int64_t B, int64_t M, int64_t T, int64_t* begin, int64_t* len, int32_t* base, int32_t* tiles, int32_t* ntiles, int64_t cap, hipStream_t stream);
+
+/* ---- rotary.hip ---- */
+/* replaces: no reference counterpart: rotary positions of q and k per document, forward and backward (the reference adds sinusoids or uses relative positions: generator/modules/_transformer/embedding.py:91-124,252-322) */
+int osp_rotary(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, int64_t in_bf16, void* qo, void* ko, int64_t out_bf16, const double* turns, const int32_t* tiles, const int32_t* ntiles, int64_t cap, const int64_t* first, int64_t Hq, int64_t Hk, int64_t D, int64_t R, int64_t interleaved, float mag, int64_t inverse, hipStream_t stream);
 
 /* ---- smallcin.hip ---- */
 /* replaces: first layers Conv2d(1, 32, (k,1)) / Conv2d(1, 32, (7,5)) and the 32-channel DiscriminatorR layers: disc/_discriminators.py:53,156-160 */

@@ -1,0 +1,454 @@
+// Group norm with an activation on packed rows, channels last: y = act(w (x - mean) rstd + b), statistics over a document's rows and a
+// group's channels, forward and backward.
+//   forward : mean, rstd per (document, group) from sum x and sum x^2
+//   backward: z = w xhat + b, dz = dy act'(z), gw = dz w;   dx = rstd (gw - mean(gw) - xhat mean(gw xhat)),
+//             dw += sum dz xhat,  db += sum dz   over all documents
+// Rows of no document get zeros (y and dx) and add nothing.
+//
+// Sums: x and x^2 are summed in 64 bits (x^2 of an f32 is exact there, so a mean far above the deviation costs nothing; the vector units
+// do 64-bit FMAs at the 32-bit rate and the kernel is bound by HBM).  The backward's per-channel sums run in 32 bits over the rows of one
+// workgroup (at most PACKED_TILE) and in 64 bits from there on.  Every sum has one fixed order: no atomics.
+//
+// Bound: HBM.  A document is larger than a CU can hold (800 rows x 256 channels x 4 bytes), so x is read twice, the second time mostly out of
+// the 256 MB last-level cache.  Forward: partial sums per (tile part, group) -> apply, whose workgroups add the few partials of their document
+// themselves (a launch of its own does it where a document has many).  Backward: per-channel partials -> per-document sums -> apply, the
+// sum of the documents' dw / db riding on the last launch.
+#include "packed_common.h"
+
+namespace {
+
+constexpr int NTH = 256, MAXC = 2048;
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
+
+// EXACT: f32 tensors take the library's expf / erff; bf16 results take one v_exp_f32 / v_rcp_f32 and the polynomial erf (<= 1.5e-7)
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float act_value(float z) {
+    if constexpr (ACT == ACT_RELU) return fmaxf(z, 0.f);
+    if constexpr (ACT == ACT_GELU) return EXACT ? gelu_f(z) : gelu_fast_f(z);
+    if constexpr (ACT == ACT_SILU) {
+        if constexpr (EXACT) return z / (1.f + expf(-z));
+        return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    }
+    return z;
+}
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float act_slope(float z) {
+    if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if constexpr (ACT == ACT_GELU) {
+        if constexpr (EXACT) {
+            const float cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+            return fmaf(z * 0.39894228040143267794f, expf(-0.5f * z * z), cdf);
+        }
+        return gelu_grad_fast_f(z);
+    }
+    if constexpr (ACT == ACT_SILU) {
+        float s;
+        if constexpr (EXACT) s = 1.f / (1.f + expf(-z)); else s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        return s * fmaf(z, 1.f - s, 1.f);
+    }
+    return 1.f;
+}
+
+struct NormArgs {
+    const void* x; int64_t ldx;
+    const void* dy; int64_t lddy;
+    const float *w, *b;
+    void* out;                                  // y or dx, (M, C) contiguous
+    float *mean, *rstd;                         // (B, G)
+    double* part;                               // forward: (slots, G, 2)
+    float* cpart;                               // backward: (slots, C, 2)
+    double* dsum;                               // backward: (B, C, 2) sums of dz, dz xhat
+    float* coef;                                // backward: (B, G, 2) mean(gw), mean(gw xhat)
+    float *dw, *db;
+    const int64_t* len;
+    const int* base;
+    const PackedTile* tiles;
+    const int* ntiles;
+    int B, C, G, cap, sub;                      // sub: parts a tile is cut into (rows PACKED_TILE / sub)
+    float eps;
+};
+
+// threads -> (row lane, channel vector): nx threads along the channels, ny rows at a time
+struct Lanes { int nx, ny, cx, ry; };
+__device__ __forceinline__ Lanes lanes_of(int nvec) {
+    Lanes l;
+    l.nx = min(nvec, NTH);
+    l.ny = NTH / l.nx;
+    l.ry = threadIdx.x / l.nx;
+    l.cx = threadIdx.x - l.ry * l.nx;
+    return l;
+}
+
+// sum over the lanes of aligned groups of L (a power of two)
+__device__ __forceinline__ double lane_group_sum(double v, int L) {
+    for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// a document's statistics from its partials; results for every group in LDS
+__device__ __forceinline__ void doc_stats(const NormArgs& p, int doc, int64_t rows, float* mean_l, float* rstd_l) {
+    const int nslots = (int)((rows + PACKED_TILE - 1) / PACKED_TILE) * p.sub;
+    const double* part = p.part + (int64_t)p.base[doc] * p.sub * p.G * 2;
+    int L = 1;
+    while (L < 64 && 2 * L * p.G <= NTH) L <<= 1;
+    const double count = (double)rows * (double)(p.C / p.G);
+    for (int g0 = 0; g0 < p.G; g0 += NTH / L) {
+        const int g = g0 + (int)threadIdx.x / L, l = threadIdx.x % L;
+        double s = 0.0, q = 0.0;
+        if (g < p.G)
+            for (int i = l; i < nslots; i += L) {
+                const double2 v = *reinterpret_cast<const double2*>(part + ((int64_t)i * p.G + g) * 2);
+                s += v.x; q += v.y;
+            }
+        s = lane_group_sum(s, L);
+        q = lane_group_sum(q, L);
+        if (g < p.G && l == 0) {
+            const double m = s / count, var = fmax(q / count - m * m, 0.0);
+            mean_l[g] = (float)m;
+            rstd_l[g] = (float)(1.0 / sqrt(var + (double)p.eps));
+        }
+    }
+    __syncthreads();
+}
+
+// ------------------------------------------------------------------------------------------------ forward: partial sums
+template <typename T, int V>
+__global__ __launch_bounds__(NTH) void gn_stats_kernel(const NormArgs p) {
+    extern __shared__ double2 smem[];           // [ny][chunk] then [C]
+    if ((int)blockIdx.x >= p.ntiles[0]) return;
+    const PackedTile tile = p.tiles[blockIdx.x];
+    const int step = PACKED_TILE / p.sub, lo = blockIdx.y * step, hi = min(tile.n, lo + step);
+    const Lanes l = lanes_of(p.C / V);
+    double2* chan = smem + NTH * V;
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row0 * p.ldx;
+    for (int c0 = 0; c0 < p.C / V; c0 += l.nx) {
+        const int cv = c0 + l.cx;
+        double s[V], q[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) { s[i] = 0.0; q[i] = 0.0; }
+        const bool on = l.ry < l.ny && cv < p.C / V;
+        if (on) {
+#pragma unroll 4
+            for (int r = lo + l.ry; r < hi; r += l.ny) {
+                float f[V];
+                PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx + cv * V);
+#pragma unroll
+                for (int i = 0; i < V; ++i) { const double d = (double)f[i]; s[i] += d; q[i] = fma(d, d, q[i]); }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) smem[(l.ry * l.nx + l.cx) * V + i] = make_double2(s[i], q[i]);
+        }
+        __syncthreads();
+        const int chunk = min(l.nx, p.C / V - c0) * V;
+        for (int c = threadIdx.x; c < chunk; c += NTH) {
+            double2 a = smem[c];
+            for (int r = 1; r < l.ny; ++r) { const double2 v = smem[r * l.nx * V + c]; a.x += v.x; a.y += v.y; }
+            chan[c0 * V + c] = a;
+        }
+        __syncthreads();
+    }
+    const int cg = p.C / p.G;
+    int L = 1;
+    while (L < 64 && 2 * L * p.G <= NTH) L <<= 1;
+    double* part = p.part + ((int64_t)(p.base[tile.doc] + tile.i0 / PACKED_TILE) * p.sub + blockIdx.y) * p.G * 2;
+    for (int g0 = 0; g0 < p.G; g0 += NTH / L) {
+        const int g = g0 + (int)threadIdx.x / L, ln = threadIdx.x % L;
+        double s = 0.0, q = 0.0;
+        if (g < p.G)
+            for (int i = ln; i < cg; i += L) { const double2 v = chan[g * cg + i]; s += v.x; q += v.y; }
+        s = lane_group_sum(s, L);
+        q = lane_group_sum(q, L);
+        if (g < p.G && ln == 0) *reinterpret_cast<double2*>(part + g * 2) = make_double2(s, q);
+    }
+}
+
+// statistics of one document per workgroup (where a document has too many partials for every apply workgroup to add them)
+__global__ __launch_bounds__(NTH) void gn_finish_kernel(const NormArgs p) {
+    __shared__ float mean_l[MAXC], rstd_l[MAXC];
+    const int doc = blockIdx.x;
+    const int64_t rows = p.len[doc];
+    if (rows <= 0) {
+        for (int g = threadIdx.x; g < p.G; g += NTH) { p.mean[(int64_t)doc * p.G + g] = 0.f; p.rstd[(int64_t)doc * p.G + g] = 0.f; }
+        return;
+    }
+    doc_stats(p, doc, rows, mean_l, rstd_l);
+    for (int g = threadIdx.x; g < p.G; g += NTH) { p.mean[(int64_t)doc * p.G + g] = mean_l[g]; p.rstd[(int64_t)doc * p.G + g] = rstd_l[g]; }
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_rows(T* y, int64_t n) {
+    for (int64_t i = threadIdx.x; i < n; i += NTH) y[i] = (T)0.f;
+}
+
+// ------------------------------------------------------------------------------------------------ forward: apply
+template <typename T, int V, int ACT, bool DIRECT>
+__global__ __launch_bounds__(NTH) void gn_apply_kernel(const NormArgs p) {
+    extern __shared__ float stat[];             // [G] mean, [G] rstd
+    if ((int)blockIdx.x >= p.ntiles[1]) return;
+    const PackedTile tile = p.tiles[blockIdx.x];
+    const int step = PACKED_TILE / p.sub, lo = blockIdx.y * step, hi = min(tile.n, lo + step);
+    if (lo >= hi) return;
+    T* y = reinterpret_cast<T*>(p.out) + (int64_t)tile.row0 * p.C;
+    if (tile.doc < 0) { zero_rows(y + (int64_t)lo * p.C, (int64_t)(hi - lo) * p.C); return; }
+    if (DIRECT) {
+        doc_stats(p, tile.doc, p.len[tile.doc], stat, stat + p.G);
+        if (tile.i0 == 0 && lo == 0)
+            for (int g = threadIdx.x; g < p.G; g += NTH) {
+                p.mean[(int64_t)tile.doc * p.G + g] = stat[g];
+                p.rstd[(int64_t)tile.doc * p.G + g] = stat[p.G + g];
+            }
+    }
+    const float* mean = DIRECT ? stat : p.mean + (int64_t)tile.doc * p.G;
+    const float* rstd = DIRECT ? stat + p.G : p.rstd + (int64_t)tile.doc * p.G;
+    const Lanes l = lanes_of(p.C / V);
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row0 * p.ldx;
+    const int cg = p.C / p.G;
+    for (int cv = l.cx; cv < p.C / V && l.ry < l.ny; cv += l.nx) {
+        float m[V], rs[V], w[V], b[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = cv * V + i, g = c / cg;
+            m[i] = mean[g]; rs[i] = rstd[g]; w[i] = p.w[c]; b[i] = p.b[c];
+        }
+#pragma unroll 4
+        for (int r = lo + l.ry; r < hi; r += l.ny) {
+            float f[V];
+            PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx + cv * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = act_value<ACT, sizeof(T) == 4>(fmaf((f[i] - m[i]) * rs[i], w[i], b[i]));
+            PackedVec<T, V>::store(y + (int64_t)r * p.C + cv * V, f);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: per-channel partial sums
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NTH) void gn_bwd_sums_kernel(const NormArgs p) {
+    __shared__ float2 stage[NTH * V];
+    if ((int)blockIdx.x >= p.ntiles[0]) return;
+    const PackedTile tile = p.tiles[blockIdx.x];
+    const int step = PACKED_TILE / p.sub, lo = blockIdx.y * step, hi = min(tile.n, lo + step);
+    const Lanes l = lanes_of(p.C / V);
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row0 * p.ldx;
+    const T* dy = reinterpret_cast<const T*>(p.dy) + (int64_t)tile.row0 * p.lddy;
+    const float *mean = p.mean + (int64_t)tile.doc * p.G, *rstd = p.rstd + (int64_t)tile.doc * p.G;
+    float2* out = reinterpret_cast<float2*>(p.cpart) + ((int64_t)(p.base[tile.doc] + tile.i0 / PACKED_TILE) * p.sub + blockIdx.y) * p.C;
+    const int cg = p.C / p.G;
+    for (int c0 = 0; c0 < p.C / V; c0 += l.nx) {
+        const int cv = c0 + l.cx;
+        if (l.ry < l.ny && cv < p.C / V) {
+            float m[V], rs[V], w[V], b[V], s[V], q[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = cv * V + i, g = c / cg;
+                m[i] = mean[g]; rs[i] = rstd[g]; w[i] = p.w[c]; b[i] = p.b[c]; s[i] = 0.f; q[i] = 0.f;
+            }
+#pragma unroll 2
+            for (int r = lo + l.ry; r < hi; r += l.ny) {
+                float f[V], d[V];
+                PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx + cv * V);
+                PackedVec<T, V>::load(d, dy + (int64_t)r * p.lddy + cv * V);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float hat = (f[i] - m[i]) * rs[i];
+                    const float dz = d[i] * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i]));
+                    s[i] += dz;
+                    q[i] = fmaf(dz, hat, q[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) stage[(l.ry * l.nx + l.cx) * V + i] = make_float2(s[i], q[i]);
+        }
+        __syncthreads();
+        const int chunk = min(l.nx, p.C / V - c0) * V;
+        for (int c = threadIdx.x; c < chunk; c += NTH) {
+            float2 a = stage[c];
+            for (int r = 1; r < l.ny; ++r) { const float2 v = stage[r * l.nx * V + c]; a.x += v.x; a.y += v.y; }
+            out[c0 * V + c] = a;
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: a document's sums
+// grid (documents, group chunks): a chunk is as many whole groups as fit 64 channels (one group where it is wider); 64 channels x 8 slot lanes
+__global__ __launch_bounds__(512) void gn_bwd_docs_kernel(const NormArgs p, int gchunk) {
+    extern __shared__ double2 chan[];           // [gchunk * C / G]
+    __shared__ double2 red[8][64];
+    const int doc = blockIdx.x, cg = p.C / p.G, g0 = blockIdx.y * gchunk, ng = min(gchunk, p.G - g0);
+    const int64_t rows = p.len[doc];
+    const int nslots = (int)((rows + PACKED_TILE - 1) / PACKED_TILE) * p.sub;
+    const float2* part = reinterpret_cast<const float2*>(p.cpart) + (int64_t)p.base[doc] * p.sub * p.C;
+    const int lane = threadIdx.x & 63, sl = threadIdx.x >> 6;
+    double2* out = reinterpret_cast<double2*>(p.dsum) + (int64_t)doc * p.C;
+    for (int c0 = 0; c0 < ng * cg; c0 += 64) {
+        const int c = c0 + lane;
+        double a = 0.0, b = 0.0;
+        if (c < ng * cg) {
+#pragma unroll 4
+            for (int i = sl; i < nslots; i += 8) { const float2 v = part[(int64_t)i * p.C + g0 * cg + c]; a += v.x; b += v.y; }
+        }
+        red[sl][lane] = make_double2(a, b);
+        __syncthreads();
+        if (sl == 0 && c < ng * cg) {
+            for (int i = 1; i < 8; ++i) { a += red[i][lane].x; b += red[i][lane].y; }
+            out[g0 * cg + c] = make_double2(a, b);
+            const double w = (double)p.w[g0 * cg + c];
+            chan[c] = make_double2(w * a, w * b);
+        }
+        __syncthreads();
+    }
+    const double inv = rows > 0 ? 1.0 / ((double)rows * (double)cg) : 0.0;
+    for (int g = threadIdx.x >> 6; g < ng; g += 8) {
+        double a = 0.0, b = 0.0;
+        for (int i = lane; i < cg; i += 64) { a += chan[g * cg + i].x; b += chan[g * cg + i].y; }
+        a = lane_group_sum(a, 64);
+        b = lane_group_sum(b, 64);
+        if (lane == 0) {
+            float* o = p.coef + ((int64_t)doc * p.G + g0 + g) * 2;
+            o[0] = (float)(a * inv);
+            o[1] = (float)(b * inv);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dx, and dw / db behind the tiles
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NTH) void gn_bwd_apply_kernel(const NormArgs p) {
+    __shared__ double2 red[4][64];
+    if ((int)blockIdx.x >= p.cap) {              // the last workgroups: 64 channels each, the documents' sums in their order
+        if (blockIdx.y) return;
+        const int lane = threadIdx.x & 63, sl = threadIdx.x >> 6, c = ((int)blockIdx.x - p.cap) * 64 + lane;
+        double a = 0.0, b = 0.0;
+        if (c < p.C) {
+#pragma unroll 4
+            for (int d = sl; d < p.B; d += 4) { const double2 v = reinterpret_cast<const double2*>(p.dsum)[(int64_t)d * p.C + c]; a += v.x; b += v.y; }
+        }
+        red[sl][lane] = make_double2(a, b);
+        __syncthreads();
+        if (sl == 0 && c < p.C) {
+            for (int i = 1; i < 4; ++i) { a += red[i][lane].x; b += red[i][lane].y; }
+            if (p.db) p.db[c] += (float)a;
+            if (p.dw) p.dw[c] += (float)b;
+        }
+        return;
+    }
+    if ((int)blockIdx.x >= p.ntiles[1] || !p.out) return;
+    const PackedTile tile = p.tiles[blockIdx.x];
+    const int step = PACKED_TILE / p.sub, lo = blockIdx.y * step, hi = min(tile.n, lo + step);
+    if (lo >= hi) return;
+    T* dx = reinterpret_cast<T*>(p.out) + (int64_t)tile.row0 * p.C;
+    if (tile.doc < 0) { zero_rows(dx + (int64_t)lo * p.C, (int64_t)(hi - lo) * p.C); return; }
+    const Lanes l = lanes_of(p.C / V);
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row0 * p.ldx;
+    const T* dy = reinterpret_cast<const T*>(p.dy) + (int64_t)tile.row0 * p.lddy;
+    const float *mean = p.mean + (int64_t)tile.doc * p.G, *rstd = p.rstd + (int64_t)tile.doc * p.G;
+    const float2* coef = reinterpret_cast<const float2*>(p.coef) + (int64_t)tile.doc * p.G;
+    const int cg = p.C / p.G;
+    for (int cv = l.cx; cv < p.C / V && l.ry < l.ny; cv += l.nx) {
+        float m[V], rs[V], w[V], b[V], c1[V], c2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = cv * V + i, g = c / cg;
+            m[i] = mean[g]; rs[i] = rstd[g]; w[i] = p.w[c]; b[i] = p.b[c];
+            const float2 k = coef[g];
+            c1[i] = k.x; c2[i] = k.y;
+        }
+#pragma unroll 2
+        for (int r = lo + l.ry; r < hi; r += l.ny) {
+            float f[V], d[V];
+            PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx + cv * V);
+            PackedVec<T, V>::load(d, dy + (int64_t)r * p.lddy + cv * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float hat = (f[i] - m[i]) * rs[i];
+                const float gw = d[i] * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i])) * w[i];
+                f[i] = rs[i] * (gw - c1[i] - hat * c2[i]);
+            }
+            PackedVec<T, V>::store(dx + (int64_t)r * p.C + cv * V, f);
+        }
+    }
+}
+
+// parts of a tile: enough workgroups to fill the chip
+int parts(int64_t M) { return M >= 65536 ? 1 : M >= 16384 ? 2 : 4; }
+
+template <typename T, int V>
+void forward(NormArgs p, int act, int64_t longest, hipStream_t s) {
+    const dim3 grid((unsigned)p.cap, (unsigned)p.sub);
+    hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(NTH), (unsigned)((NTH * V + p.C) * sizeof(double2)), s, p);
+    const bool direct = cdiv(longest, PACKED_TILE) * p.sub * p.G <= 2048;
+    if (!direct) hipLaunchKernelGGL(gn_finish_kernel, dim3((unsigned)p.B), dim3(NTH), 0, s, p);
+#define A(ACT_)                                                                                                                                 \
+    if (direct) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_, true>), grid, dim3(NTH), (unsigned)(2 * p.G * sizeof(float)), s, p);             \
+    else hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_, false>), grid, dim3(NTH), 0, s, p)
+    if (act == ACT_RELU) { A(ACT_RELU); } else if (act == ACT_GELU) { A(ACT_GELU); } else if (act == ACT_SILU) { A(ACT_SILU); } else { A(ACT_NONE); }
+#undef A
+}
+
+template <typename T, int V>
+void backward(NormArgs p, int act, hipStream_t s) {
+    const dim3 grid((unsigned)p.cap, (unsigned)p.sub), grid2((unsigned)(p.cap + cdiv(p.C, 64)), (unsigned)p.sub);
+    const int cg = p.C / p.G, gchunk = cg >= 64 ? 1 : 64 / cg;
+#define A(ACT_)                                                                                                                                 \
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT_>), grid, dim3(NTH), 0, s, p);                                                              \
+    hipLaunchKernelGGL(gn_bwd_docs_kernel, dim3((unsigned)p.B, (unsigned)cdiv(p.G, gchunk)), dim3(512), (unsigned)(gchunk * cg * sizeof(double2)), s, p, gchunk); \
+    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT_>), grid2, dim3(NTH), 0, s, p)
+    if (act == ACT_RELU) { A(ACT_RELU); } else if (act == ACT_GELU) { A(ACT_GELU); } else if (act == ACT_SILU) { A(ACT_SILU); } else { A(ACT_NONE); }
+#undef A
+}
+
+}  // namespace
+
+// Bytes of the workspace of one call (forward or backward).
+extern "C" int64_t osp_group_norm_workspace_bytes(int64_t B, int64_t M, int64_t C, int64_t G, int64_t backward) {
+    if (B <= 0 || M < 0 || C <= 0 || G <= 0) return 0;
+    const int64_t slots = (M / PACKED_TILE + B) * parts(M);
+    if (!backward) return slots * G * 16 + 256;
+    return slots * C * 8 + B * C * 16 + B * G * 8 + 512;
+}
+
+extern "C" int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, void* y, float* mean, float* rstd,
+                                  void* workspace, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles,
+                                  int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, float eps, int64_t act,
+                                  hipStream_t stream) {
+    OSP_CHECK_ARG(x && w && b && y && mean && rstd && workspace && len && base && tiles && ntiles, "null pointer");
+    OSP_CHECK_ARG(B > 0 && M > 0 && longest > 0 && C > 0 && C <= MAXC && G > 0 && C % G == 0 && ldx >= C, "channels (at most 2048) must be a multiple of groups");
+    OSP_CHECK_ARG(eps > 0.f && act >= ACT_NONE && act <= ACT_SILU && cap > 0 && cap < (int64_t)1 << 30 && packed_aligned(workspace, 16), "bad eps, activation or workspace");
+    NormArgs p = {};
+    p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.out = y; p.mean = mean; p.rstd = rstd; p.part = reinterpret_cast<double*>(workspace);
+    p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
+    p.B = (int)B; p.C = (int)C; p.G = (int)G; p.cap = (int)cap; p.sub = parts(M); p.eps = eps;
+    const int V = bf16 ? 8 : 4;
+    const bool wide = C % V == 0 && ldx % V == 0 && packed_aligned(x, 16) && packed_aligned(y, 16);
+    if (bf16) { if (wide) forward<__bf16, 8>(p, (int)act, longest, stream); else forward<__bf16, 1>(p, (int)act, longest, stream); }
+    else { if (wide) forward<float, 4>(p, (int)act, longest, stream); else forward<float, 1>(p, (int)act, longest, stream); }
+    OSP_LAUNCH_CHECK();
+    return OSP_OK;
+}
+
+extern "C" int osp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b,
+                                  const float* mean, const float* rstd, void* dx, float* dw, float* db, void* workspace, const int64_t* len,
+                                  const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M,
+                                  int64_t C, int64_t G, int64_t act, hipStream_t stream) {
+    OSP_CHECK_ARG(dy && x && w && b && mean && rstd && workspace && len && base && tiles && ntiles, "null pointer");
+    OSP_CHECK_ARG(B > 0 && M > 0 && C > 0 && C <= MAXC && G > 0 && C % G == 0 && ldx >= C && lddy >= C, "channels (at most 2048) must be a multiple of groups");
+    OSP_CHECK_ARG(act >= ACT_NONE && act <= ACT_SILU && cap > 0 && cap < (int64_t)1 << 30 && packed_aligned(workspace, 16), "bad activation or workspace");
+    NormArgs p = {};
+    p.x = x; p.ldx = ldx; p.dy = dy; p.lddy = lddy; p.w = w; p.b = b; p.out = dx;
+    p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd); p.dw = dw; p.db = db;
+    p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
+    p.B = (int)B; p.C = (int)C; p.G = (int)G; p.cap = (int)cap; p.sub = parts(M);
+    const int64_t slots = (M / PACKED_TILE + B) * p.sub;
+    char* ws = reinterpret_cast<char*>(workspace);
+    p.dsum = reinterpret_cast<double*>(ws);                            // (B, C, 2) f64
+    p.cpart = reinterpret_cast<float*>(ws + B * C * 16);               // (slots, C, 2) f32
+    p.coef = reinterpret_cast<float*>(ws + B * C * 16 + slots * C * 8);
+    const int V = bf16 ? 8 : 4;
+    const bool wide = C % V == 0 && ldx % V == 0 && lddy % V == 0 && packed_aligned(x, 16) && packed_aligned(dy, 16) && packed_aligned(dx, 16);
+    if (bf16) { if (wide) backward<__bf16, 8>(p, (int)act, stream); else backward<__bf16, 1>(p, (int)act, stream); }
+    else { if (wide) backward<float, 4>(p, (int)act, stream); else backward<float, 1>(p, (int)act, stream); }
+    OSP_LAUNCH_CHECK();
+    return OSP_OK;
+}

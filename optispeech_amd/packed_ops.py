@@ -1,0 +1,219 @@
+"""Operators on packed rows: a batch of ragged utterances as one table of rows, without padding.
+
+``PackedRows`` says which rows of a table (M, ...) form which document; rotary positions restart in every document, group norm takes its
+statistics over a document's rows, attention stays inside a document.  A padded batch (B, T, ...) flattened to (B * T, ...) is the same thing
+with gaps.  Rows of no document -- a padded tail, the rows behind the last offset -- come out as zeros, in gradients too, whatever
+they hold on the way in.
+
+The handle is built once per batch from device offsets or lengths (no copy to the host) and used by every layer and direction.
+Like the rest of the package: kernels go to torch's current stream on the current device, parameter gradients are accumulated into
+``param.grad`` by the kernels, activations flow through autograd.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import precision as _precision
+from ._lib import OspError, call, lib
+from .ops import _grad_aware, _saving, _want, gsink
+
+ACTS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _refuse(cond, msg):
+    if cond:
+        raise OspError(msg)
+
+
+def _size(name, *args):
+    f = getattr(lib().cdll, name)
+    f.restype = ctypes.c_int64
+    return f(*(ctypes.c_int64(int(a)) for a in args))
+
+
+class PackedRows:
+    """Documents of a table of ``rows`` rows: ``begin`` / ``length`` (docs,) int64 on the device, the tile list of the kernels, and the
+    host's upper bound ``longest`` on a document's length."""
+
+    def __init__(self, src, padded, docs, rows, longest):
+        _refuse(src.dtype != torch.int64 or src.dim() != 1 or not src.is_contiguous(), "offsets / lengths must be a contiguous 1-D int64 tensor")
+        _refuse(not src.is_cuda, "offsets / lengths must live on the GPU")
+        _refuse(docs < 1 or rows < 0 or longest < 0, f"a batch needs at least one document (docs {docs}, rows {rows}, longest {longest})")
+        self.docs, self.rows, self.longest, self.device = docs, rows, min(longest, rows), src.device
+        self.cap = _size("osp_packed_rows_tiles", docs, rows)
+        long = torch.empty((2, docs), device=src.device, dtype=torch.int64)
+        ints = torch.empty((4 * self.cap + docs + 2,), device=src.device, dtype=torch.int32)
+        self.begin, self.length = long[0], long[1]
+        self.tiles, self.base, self.ntiles = ints[:4 * self.cap], ints[4 * self.cap:4 * self.cap + docs], ints[4 * self.cap + docs:]
+        call("osp_packed_rows_plan", src, int(padded), docs, rows, rows // docs if padded else 0, self.begin, self.length, self.base, self.tiles,
+             self.ntiles, self.cap)
+
+    @classmethod
+    def from_offsets(cls, offsets, rows, longest=None):
+        """Document b owns the rows [offsets[b], offsets[b + 1]) of a table of ``rows`` rows.  offsets (docs + 1,) int64 on the GPU, ascending
+        (clamped to the table; one below its predecessor counts as its predecessor).  ``longest``: the host's bound on a document's
+        length; without it the table's rows, which is always right and costs launches sized for one document that long."""
+        return cls(offsets, False, offsets.numel() - 1, int(rows), int(rows if longest is None else longest))
+
+    @classmethod
+    def from_padded(cls, lengths, T):
+        """Document b owns the first lengths[b] (clamped to 0 .. T) of its T rows in a (docs * T, ...) table."""
+        return cls(lengths, True, lengths.numel(), lengths.numel() * int(T), int(T))
+
+    def _check(self, t, name):
+        _refuse(t.shape[0] != self.rows, f"{name} has {t.shape[0]} rows, the documents were laid out for {self.rows}")
+        _refuse(t.device != self.device, f"{name} is on {t.device}, the documents on {self.device}")
+
+
+# ------------------------------------------------------------------------------------------------------------------ rotary positions
+class Rotary:
+    """Frequencies of rotary positions, f_i = base^(-2 i / channels), and their scaling for contexts longer than ``original_length``:
+
+    ``none``; ``linear``: f_i / factor; ``base``: the base grows to base * factor^(channels / (channels - 2)), so that the slowest pair is
+    slowed by the factor and the fastest is left; ``parts``: a pair that makes at least ``fast`` turns within the original length keeps f_i, one
+    that makes at most ``slow`` turns gets f_i / factor, those between a blend, linear in the turns; results are scaled by
+    1 + 0.1 ln factor."""
+
+    def __init__(self, channels, base=10000.0, layout="half", scaling="none", factor=1.0, original_length=None, slow=1.0, fast=32.0,
+                 device="cuda"):
+        _refuse(channels < 2 or channels % 2, f"an even number of channels turns, not {channels}")
+        _refuse(layout not in ("half", "interleaved"), f"layout {layout!r}: 'half' or 'interleaved'")
+        _refuse(scaling not in ("none", "linear", "base", "parts"), f"scaling {scaling!r}: 'none', 'linear', 'base' or 'parts'")
+        _refuse(scaling != "none" and not factor >= 1.0, f"a context is stretched by a factor >= 1, not {factor}")
+        _refuse(scaling == "base" and channels == 2, "a single pair has no slower one for the base to act on")
+        _refuse(scaling == "parts" and (original_length is None or not fast > slow), "scaling 'parts' needs original_length and fast > slow")
+        _refuse(not base > 0.0, f"base {base}")
+        self.channels, self.layout, self.magnitude = int(channels), layout, 1.0
+        if scaling == "base":
+            base = base * factor ** (channels / (channels - 2))
+        f = [base ** (-2.0 * i / channels) for i in range(channels // 2)]
+        if scaling == "linear":
+            f = [x / factor for x in f]
+        elif scaling == "parts":
+            def blend(x):
+                keep = min(1.0, max(0.0, (original_length * x / (2.0 * math.pi) - slow) / (fast - slow)))
+                return x * keep + x / factor * (1.0 - keep)
+            f = [blend(x) for x in f]
+            self.magnitude = 1.0 + 0.1 * math.log(factor)
+        #: turns per position, 64 bits: the kernel forms angles from it (csrc/rotary.hip)
+        self.turns = torch.tensor([x / (2.0 * math.pi) for x in f], dtype=torch.float64, device=device)
+
+
+def _heads(t, name):
+    """(M, heads, width) with contiguous channels; any row and head stride."""
+    _refuse(t.dim() != 3, f"{name} must be (rows, heads, width), not {tuple(t.shape)}")
+    _refuse(t.dtype not in (torch.float32, torch.bfloat16), f"{name}: float32 or bfloat16, not {t.dtype}")
+    _refuse(not t.is_cuda, f"{name} must live on the GPU")
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _rotate(q, k, rope, rows, first, out_dtype, inverse):
+    q, k = _heads(q, "q"), _heads(k, "k")
+    qo = torch.empty(q.shape, device=q.device, dtype=out_dtype)
+    ko = torch.empty(k.shape, device=k.device, dtype=out_dtype)
+    if q.shape[0]:
+        call("osp_rotary", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), int(q.dtype == torch.bfloat16), qo, ko,
+             int(out_dtype == torch.bfloat16), rope.turns, rows.tiles, rows.ntiles, rows.cap, first, q.shape[1], k.shape[1], q.shape[2],
+             rope.channels, int(rope.layout == "interleaved"), float(rope.magnitude), int(inverse))
+    return qo, ko
+
+
+class RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, rope, rows, first, out_dtype):
+        ctx.cfg = (rope, rows, first, q.dtype)
+        ctx.shapes = (q.shape, k.shape, out_dtype, q.device)
+        return _rotate(q, k, rope, rows, first, out_dtype, False)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        rope, rows, first, dtype = ctx.cfg
+        qs, ks, od, dev = ctx.shapes
+        dq = torch.zeros(qs, device=dev, dtype=od) if dq is None else dq.to(od)
+        dk = torch.zeros(ks, device=dev, dtype=od) if dk is None else dk.to(od)
+        gq, gk = _rotate(dq, dk, rope, rows, first, dtype, True)
+        return gq, gk, None, None, None, None
+
+
+def rotary(q, k, rope, rows, first=None, out_dtype=None):
+    """Turn the first ``rope.channels`` channels of every head of q (M, heads, width) and k (M, shared, width) by the row's position: its index in
+    its document plus ``first`` (docs,) int64 (the frames already in a cache).  One launch; results are contiguous, in ``out_dtype`` (float32
+    or bfloat16; the inputs' type without it).  The gradient is the inverse turn, in the inputs' type."""
+    _refuse(q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] < 1 or k.shape[1] < 1,
+            f"q {tuple(q.shape)} and k {tuple(k.shape)} must be (rows, heads, width) with the same rows and width")
+    _refuse(q.dtype != k.dtype, f"q is {q.dtype}, k {k.dtype}")
+    out_dtype = q.dtype if out_dtype is None else out_dtype
+    _refuse(out_dtype not in (torch.float32, torch.bfloat16), f"out_dtype: float32 or bfloat16, not {out_dtype}")
+    _refuse(rope.channels > q.shape[2], f"{rope.channels} turned channels in heads of {q.shape[2]}")
+    _refuse(rope.turns.device != q.device, f"the frequencies are on {rope.turns.device}, q on {q.device}")
+    rows._check(q, "q")
+    rows._check(k, "k")
+    if first is not None:
+        _refuse(first.dtype != torch.int64 or first.shape != (rows.docs,) or not first.is_contiguous() or first.device != q.device,
+                "first must be a contiguous (docs,) int64 tensor on q's device")
+    return RotaryFn.apply(q, k, rope, rows, first, out_dtype)
+
+
+# ------------------------------------------------------------------------------------------------------------------ group norm
+def _matrix(t, name):
+    _refuse(t.dim() != 2, f"{name} must be (rows, channels), not {tuple(t.shape)}")
+    _refuse(t.dtype not in (torch.float32, torch.bfloat16), f"{name}: float32 or bfloat16, not {t.dtype}")
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _workspace(nbytes, device):
+    # one per call, from the caching allocator: two captured graphs never share one
+    return torch.empty((nbytes,), device=device, dtype=torch.uint8)
+
+
+@_grad_aware
+class GroupNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, groups, rows, eps, act):
+        M, C = x.shape
+        x = _matrix(x, "x")
+        y = torch.empty((M, C), device=x.device, dtype=x.dtype)
+        stats = torch.empty((2, rows.docs, groups), device=x.device, dtype=torch.float32)
+        if M and rows.longest:
+            ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 0), x.device)
+            call("osp_group_norm_fwd", x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, y, stats[0], stats[1], ws, rows.length, rows.base,
+                 rows.tiles, rows.ntiles, rows.cap, rows.docs, M, rows.longest, C, groups, float(eps), act)
+        else:
+            y.zero_()
+        if _saving(ctx):
+            ctx.save_for_backward(x, stats)
+            ctx.params, ctx.cfg = (w, b), (groups, rows, act)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, stats = ctx.saved_tensors
+        (w, b), (groups, rows, act) = ctx.params, ctx.cfg
+        M, C = x.shape
+        dy = _matrix(dy, "dy")
+        dx = torch.empty((M, C), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
+        if M and rows.longest:
+            ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 1), x.device)
+            call("osp_group_norm_bwd", dy, dy.stride(0), x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, stats[0], stats[1], dx,
+                 gsink(w) if _want(w) else None, gsink(b) if _want(b) else None, ws, rows.length, rows.base, rows.tiles, rows.ntiles, rows.cap,
+                 rows.docs, M, C, groups, act)
+        elif dx is not None:
+            dx.zero_()
+        return dx, None, None, None, None, None, None
+
+
+def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
+    """act(weight * (x - mean) / sqrt(var + eps) + bias), mean and variance over a document's rows and a group's channels.  x (M, C) float32
+    or bfloat16 (any row stride), weight / bias (C,) float32, act None, "relu", "gelu" (with erf) or "silu"; C <= 2048."""
+    _refuse(x.dim() != 2 or not x.is_cuda, "x must be a (rows, channels) tensor on the GPU")
+    _refuse(x.dtype not in (torch.float32, torch.bfloat16), f"x: float32 or bfloat16, not {x.dtype}")
+    C = x.shape[1]
+    _refuse(groups < 1 or C < 1 or C % groups or C > 2048, f"{C} channels (at most 2048) do not divide into {groups} groups")
+    _refuse(act not in ACTS, f"act {act!r}: one of {sorted(a for a in ACTS if a)} or None")
+    _refuse(not eps > 0.0, f"eps {eps}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        _refuse(t.shape != (C,) or t.dtype != torch.float32 or not t.is_contiguous() or t.device != x.device,
+                f"{name} must be a contiguous ({C},) float32 tensor on x's device")
+    rows._check(x, "x")
+    return GroupNormFn.apply(x, weight, bias, int(groups), rows, float(eps), ACTS[act])

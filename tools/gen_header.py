@@ -137,6 +137,14 @@ REPLACES = {
     "osp_sum_scaled": "torch.mean over the per-utterance loss terms: generator/loss.py:190-193, alignments.py:236-238",
     "osp_dot_multi": "weighted loss sums: generator/__init__.py:175-181, vocoder/wavenext/disc/__init__.py:105-111",
     "osp_scale_vec": "autograd of the weighted loss sums",
+    "osp_packed_rows_tiles": "no reference counterpart: most tiles the tile list of a packed batch can have (the reference pads every batch)",
+    "osp_packed_rows_plan": "no reference counterpart: documents and tile list of a packed or padded batch, from offsets / lengths on the device",
+    "osp_rotary": "no reference counterpart: rotary positions of q and k per document, forward and backward (the reference adds sinusoids or uses "
+                  "relative positions: generator/modules/_transformer/embedding.py:91-124,252-322)",
+    "osp_group_norm_workspace_bytes": "workspace query for osp_group_norm_fwd / osp_group_norm_bwd",
+    "osp_group_norm_fwd": "no reference counterpart: group norm + activation over the rows of each document (the place of BatchNorm + swish in "
+                          "_conformer/convolution.py:61-70, which counts padded frames)",
+    "osp_group_norm_bwd": "autograd of the same",
     "osp_source_hash": "content hash of the sources this library was built from (optispeech_amd/build.py checks it; no reference counterpart)",
 }
 
