@@ -1,0 +1,276 @@
+// Attention over documents, backward: probabilities are recomputed tile by tile from q, k and the log2-sum-exp of the forward.
+//   P = exp2(s - lse),  dP = dO V^T,  delta_i = sum_d dO_id O_id  (= sum_j P dP),  dS = P (dP - delta) (1 - tanh^2)
+//   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO;   dK and dV of a shared key head are summed over its query heads
+// Scores and masks: attention_packed_common.h.  Two kernels, no atomics, every sum in one fixed order:
+//   dq : a wave owns 32 queries and walks the keys (S^T and dP^T per tile, dQ^T += K^T dS^T);  it also writes delta
+//   dkv: a wave owns 32 keys with K and V fragments in registers and walks the queries of every head of its group (S and dP, dV^T += dO^T P,
+//        dK^T += Q^T dS): the sum over shared heads stays in its accumulators
+// S and dP are computed twice, 7 instead of 5 products per tile pair: the price of combining dQ without atomics or a partial dQ per key tile.
+#include "attention_packed_common.h"
+
+namespace {
+using namespace pattn;
+
+// ------------------------------------------------------------------------------------------------ dQ and delta
+template <typename T, int DP, int MODE>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_kernel(const Args p) {
+    typedef Op<T> O;
+    constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32, ROW = DP * (int)sizeof(T) + 16;
+    constexpr bool EXACT = sizeof(T) == 4;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][KT * ROW];
+    const int h = blockIdx.x % p.Hq, ti = blockIdx.x / p.Hq;
+    if (ti >= p.ntiles[1]) return;
+    const PackedTile tile = p.tiles[ti];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
+    const int w0 = wave * 32, qi = w0 + l31;
+    const int64_t qrow = (int64_t)tile.row0 + qi;
+    T* out = reinterpret_cast<T*>(p.dq) + (qrow * p.Hq + h) * p.D;
+    if (tile.doc < 0) {
+        if (qi < tile.n)
+            for (int d = half * 8; d < p.D; d += 16)
+                for (int e = 0; e < 8; ++e) out[d + e] = (T)0.f;
+        return;
+    }
+    const int qlen = (int)p.qlen[tile.doc], klen = (int)p.klen[tile.doc];
+    const int prefix = p.prefix ? (int)min(max(p.prefix[tile.doc], (int64_t)0), (int64_t)klen) : 0;
+    const int64_t kb = p.kbegin[tile.doc];
+    const int hk = h / p.G;
+    const T* kp = reinterpret_cast<const T*>(p.k) + kb * p.kr + (int64_t)hk * p.kh;
+    const T* vp = reinterpret_cast<const T*>(p.v) + kb * p.vr + (int64_t)hk * p.vh;
+    const int off = klen - qlen + tile.i0;
+    const int pos = off + qi, lim = qi < tile.n ? key_limit(pos, klen, prefix, p.causal) : 0;
+    const int kmax = max(key_limit(off + tile.n - 1, klen, prefix, p.causal), 0);
+    const int wmax = w0 < tile.n ? max(key_limit(off + min(w0 + 31, tile.n - 1), klen, prefix, p.causal), 0) : 0;
+    const int wmin = key_limit(off + w0, klen, prefix, p.causal);
+    const bool on = qi < tile.n;
+    typename O::Frag qf[O::template NF<DP>], dof[O::template NF<DP>];
+    load_frags<T, DP>(dof, reinterpret_cast<const T*>(p.dout) + qrow * p.dor + (int64_t)h * p.doh, on, p.D, half);
+    float delta = 0.f;
+    {
+        load_frags<T, DP>(qf, reinterpret_cast<const T*>(p.o) + (qrow * p.Hq + h) * p.D, on, p.D, half);   // o, then q
+#pragma unroll
+        for (int s = 0; s < O::template NF<DP>; ++s)
+#pragma unroll
+            for (int e = 0; e < O::EPC; ++e) delta = fmaf((float)dof[s][e], (float)qf[s][e], delta);
+        delta = half_sum(delta);
+        if (on && half == 0) p.delta[(int64_t)h * p.Mq + qrow] = delta;
+    }
+    load_frags<T, DP>(qf, reinterpret_cast<const T*>(p.q) + qrow * p.qr + (int64_t)h * p.qh, on, p.D, half);
+    const float lse = on ? p.lse[(int64_t)h * p.Mq + qrow] : EMPTY;
+    const Score sc = make_score<MODE, EXACT>(p, h);
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    const int nt = (kmax + KT - 1) / KT;
+    Stage<T, DP, KT, 256> ks, vs;
+    if (nt > 0) {
+        ks.load(kp, p.kr, 0, klen, p.D, tid);
+        vs.load(vp, p.vr, 0, klen, p.D, tid);
+        ks.store(lds[0][0], tid);
+        vs.store(lds[0][1], tid);
+        if (nt > 1) { ks.load(kp, p.kr, KT, klen, p.D, tid); vs.load(vp, p.vr, KT, klen, p.D, tid); }
+    }
+    __syncthreads();
+    for (int t = 0; t < nt; ++t) {
+        const int k0 = t * KT;
+        const char *kl = lds[t & 1][0], *vl = lds[t & 1][1];
+        if (k0 < wmax) {
+            const float dist = (float)(pos - k0 - 4 * half);
+            const bool masked = k0 + KT > wmin;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                f32x16 st = O::template score<DP>(kl + b * 32 * ROW, qf, l31, half);
+                const f32x16 dp = O::template score<DP>(vl + b * 32 * ROW, dof, l31, half);
+                typename O::Cols ds;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float g, s = sc.template value_and_slope<MODE, EXACT>(st[i], dist - (float)(b * 32 + (i >> 2) * 8 + (i & 3)), g);
+                    if (masked) s = k0 + b * 32 + (i >> 2) * 8 + 4 * half + (i & 3) < lim ? s : -INFINITY;
+                    O::set(ds, i, __builtin_amdgcn_exp2f(s - lse) * (dp[i] - delta) * g);
+                }
+                O::template value<DP>(acc, ds, kl + b * 32 * ROW, lane);
+            }
+        }
+        if (t + 1 < nt) {
+            ks.store(lds[(t + 1) & 1][0], tid);
+            vs.store(lds[(t + 1) & 1][1], tid);
+            if (t + 2 < nt) { ks.load(kp, p.kr, k0 + 2 * KT, klen, p.D, tid); vs.load(vp, p.vr, k0 + 2 * KT, klen, p.D, tid); }
+        }
+        __syncthreads();
+    }
+    if (!on) return;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = d * 32 + g * 8 + 4 * half;
+            const float r[4] = {acc[d][4 * g] * p.scale, acc[d][4 * g + 1] * p.scale, acc[d][4 * g + 2] * p.scale, acc[d][4 * g + 3] * p.scale};
+            if (c < p.D) PackedVec<T, 4>::store(out + c, r);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+template <typename T, int DP, int MODE>
+__global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(const Args p) {
+    typedef Op<T> O;
+    constexpr int QT = 32, ROW = DP * (int)sizeof(T) + 16;
+    constexpr bool EXACT = sizeof(T) == 4;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][QT * ROW];                  // [buffer][Q, dO]
+    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];                      // [buffer][log2-sum-exp, delta]
+    const int hk = blockIdx.x % p.Hk, ti = blockIdx.x / p.Hk;
+    if (ti >= p.ntiles[1]) return;
+    const PackedTile tile = p.tiles[ti];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
+    const int w0 = wave * 32, ki = w0 + l31;
+    const int64_t krow = (int64_t)tile.row0 + ki;
+    const bool on = ki < tile.n;
+    T* outk = reinterpret_cast<T*>(p.dk) + (krow * p.Hk + hk) * p.D;
+    T* outv = reinterpret_cast<T*>(p.dv) + (krow * p.Hk + hk) * p.D;
+    if (tile.doc < 0) {
+        if (on)
+            for (int d = half * 8; d < p.D; d += 16)
+                for (int e = 0; e < 8; ++e) { outk[d + e] = (T)0.f; outv[d + e] = (T)0.f; }
+        return;
+    }
+    const int qlen = (int)p.qlen[tile.doc], klen = (int)p.klen[tile.doc];
+    const int prefix = p.prefix ? (int)min(max(p.prefix[tile.doc], (int64_t)0), (int64_t)klen) : 0;
+    const int64_t qb = p.qbegin[tile.doc];
+    const int off = klen - qlen;                                                       // position of the document's first query
+    // first query that sees a key of the tile: all see the prefix, key j is seen from position j on
+    const int first = !p.causal || tile.i0 < prefix ? 0 : max(tile.i0 - off, 0);
+    typename O::Frag kf[O::template NF<DP>], vf[O::template NF<DP>];
+    load_frags<T, DP>(kf, reinterpret_cast<const T*>(p.k) + krow * p.kr + (int64_t)hk * p.kh, on, p.D, half);
+    load_frags<T, DP>(vf, reinterpret_cast<const T*>(p.v) + krow * p.vr + (int64_t)hk * p.vh, on, p.D, half);
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
+    const int key = tile.i0 + ki;                                                      // this lane's key in the document
+    const int nqt = first < qlen ? (qlen - first + QT - 1) / QT : 0, nt = nqt * p.G;
+    Stage<T, DP, QT, 256> qs, dos;
+    float st_reg = 0.f;
+    auto load = [&](int t) {
+        const int h = hk * p.G + t / nqt, r0 = first + (t % nqt) * QT;
+        qs.load(reinterpret_cast<const T*>(p.q) + qb * p.qr + (int64_t)h * p.qh, p.qr, r0, qlen, p.D, tid);
+        dos.load(reinterpret_cast<const T*>(p.dout) + qb * p.dor + (int64_t)h * p.doh, p.dor, r0, qlen, p.D, tid);
+        if (tid < 2 * QT) {
+            const int r = r0 + (tid & (QT - 1));
+            const float* src = tid < QT ? p.lse : p.delta;
+            st_reg = r < qlen ? src[(int64_t)h * p.Mq + qb + r] : tid < QT ? EMPTY : 0.f;
+        }
+    };
+    auto store = [&](int buf) {
+        qs.store(lds[buf][0], tid);
+        dos.store(lds[buf][1], tid);
+        if (tid < 2 * QT) stat[buf][tid / QT][tid & (QT - 1)] = st_reg;
+    };
+    if (nt > 0) {
+        load(0);
+        store(0);
+        if (nt > 1) load(1);
+    }
+    __syncthreads();
+    Score sc = make_score<MODE, EXACT>(p, hk * p.G);
+    for (int t = 0; t < nt; ++t) {
+        const int buf = t & 1, r0 = first + (t % nqt) * QT;
+        if constexpr (MODE & SLOPE) sc.slope2 = p.slopes[hk * p.G + t / nqt] * LOG2E;
+        const char *ql = lds[buf][0], *dl = lds[buf][1];
+        const int pos0 = off + r0;
+        // the wave's keys are all behind the tile's last query: nothing seen
+        const bool seen = !p.causal || tile.i0 + w0 < prefix || pos0 + QT - 1 >= tile.i0 + w0;
+        if (w0 < tile.n && seen) {
+            const f32x16 sr = O::template score<DP>(ql, kf, l31, half);
+            const f32x16 dp = O::template score<DP>(dl, vf, l31, half);
+            const float dist = (float)(pos0 + 4 * half - key);
+            const int row_min = key < prefix ? -0x40000000 : key - pos0 - 4 * half;     // rows (4 half taken off) from here on see the key
+            const bool masked = p.causal && pos0 < tile.i0 + w0 + 31;
+            typename O::Cols pc, ds;
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[buf][0][g4 * 8 + 4 * half]);
+                const f32x4 del = *reinterpret_cast<const f32x4*>(&stat[buf][1][g4 * 8 + 4 * half]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = g4 * 4 + e;
+                    float g, s = sc.template value_and_slope<MODE, EXACT>(sr[i], dist + (float)(g4 * 8 + e), g);
+                    if (masked) s = g4 * 8 + e >= row_min ? s : -INFINITY;
+                    const float pr = __builtin_amdgcn_exp2f(s - lse[e]);
+                    O::set(pc, i, pr);
+                    O::set(ds, i, pr * (dp[i] - del[e]) * g);
+                }
+            }
+            O::template value<DP>(dv, pc, dl, lane);
+            O::template value<DP>(dk, ds, ql, lane);
+        }
+        if (t + 1 < nt) {
+            store(buf ^ 1);
+            if (t + 2 < nt) load(t + 2);
+        }
+        __syncthreads();
+    }
+    if (!on) return;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = d * 32 + g * 8 + 4 * half;
+            const float a[4] = {dk[d][4 * g] * p.scale, dk[d][4 * g + 1] * p.scale, dk[d][4 * g + 2] * p.scale, dk[d][4 * g + 3] * p.scale};
+            const float b[4] = {dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+            if (c < p.D) { PackedVec<T, 4>::store(outk + c, a); PackedVec<T, 4>::store(outv + c, b); }
+        }
+}
+
+template <typename T, int DP>
+void launch(Args p, const PackedTile* ktiles, const int* kntiles, int kcap, hipStream_t s) {
+    const int mode = (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0);
+    Args pk = p;
+    pk.tiles = ktiles; pk.ntiles = kntiles; pk.cap_tiles = kcap;
+    const dim3 gq((unsigned)(p.cap_tiles * p.Hq)), gk((unsigned)(kcap * p.Hk));
+#define L(M_)                                                                                       \
+    hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, M_>), gq, dim3(256), 0, s, p);                  \
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, M_>), gk, dim3(256), 0, s, pk)
+    if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else { L(3); }
+#undef L
+}
+template <typename T>
+void launch_width(const Args& p, const PackedTile* kt, const int* kn, int kcap, hipStream_t s) {
+    switch (padded_width(p.D)) {
+        case 32: launch<T, 32>(p, kt, kn, kcap, s); break;
+        case 64: launch<T, 64>(p, kt, kn, kcap, s); break;
+        case 96: launch<T, 96>(p, kt, kn, kcap, s); break;
+        default: launch<T, 128>(p, kt, kn, kcap, s);
+    }
+}
+}  // namespace
+
+extern "C" int osp_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                                        int64_t v_row, int64_t v_head, const void* o, const float* lse, const void* dout, int64_t do_row,
+                                        int64_t do_head, int64_t bf16, void* dq, void* dk, void* dv, float* delta, const int64_t* qbegin,
+                                        const int64_t* qlen, const int32_t* qtiles, const int32_t* qntiles, int64_t qcap, const int64_t* kbegin,
+                                        const int64_t* klen, const int32_t* ktiles, const int32_t* kntiles, int64_t kcap, const int64_t* prefix,
+                                        const float* slopes, int64_t Mq, int64_t Hq, int64_t Hk, int64_t D, float scale, float softcap, int64_t causal,
+                                        hipStream_t stream) {
+    OSP_CHECK_ARG(q && k && v && o && lse && dout && dq && dk && dv && delta && qbegin && qlen && qtiles && qntiles && kbegin && klen && ktiles && kntiles,
+                  "null pointer");
+    OSP_CHECK_ARG(Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq <= 65536, "query heads must be a multiple of the key heads");
+    OSP_CHECK_ARG(D > 0 && D <= 128 && D % 8 == 0, "head width must be a multiple of 8, at most 128");
+    const int E = bf16 ? 8 : 4;
+    OSP_CHECK_ARG(q_row % E == 0 && q_head % E == 0 && k_row % E == 0 && k_head % E == 0 && v_row % E == 0 && v_head % E == 0 && do_row % E == 0 &&
+                  do_head % E == 0 && packed_aligned(q, 16) && packed_aligned(k, 16) && packed_aligned(v, 16) && packed_aligned(dout, 16) &&
+                  packed_aligned(o, 16) && packed_aligned(dq, 16) && packed_aligned(dk, 16) && packed_aligned(dv, 16), "rows and heads must start on 16 bytes");
+    OSP_CHECK_ARG(qcap > 0 && kcap > 0 && qcap * Hq < (int64_t)1 << 31 && kcap * Hk < (int64_t)1 << 31 && softcap >= 0.f && (causal || !prefix),
+                  "bad tile list, cap or mask");
+    Args p = {};
+    p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv; p.lse = const_cast<float*>(lse); p.delta = delta;
+    p.qr = q_row; p.qh = q_head; p.kr = k_row; p.kh = k_head; p.vr = v_row; p.vh = v_head; p.dor = do_row; p.doh = do_head;
+    p.qbegin = qbegin; p.qlen = qlen; p.kbegin = kbegin; p.klen = klen; p.tiles = reinterpret_cast<const PackedTile*>(qtiles); p.ntiles = qntiles;
+    p.prefix = prefix; p.slopes = slopes; p.Mq = Mq; p.cap_tiles = (int)qcap; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk); p.D = (int)D;
+    p.causal = (int)(causal != 0); p.scale = scale; p.softcap = softcap;
+    const PackedTile* kt = reinterpret_cast<const PackedTile*>(ktiles);
+    if (bf16) launch_width<__bf16>(p, kt, kntiles, (int)kcap, stream); else launch_width<float>(p, kt, kntiles, (int)kcap, stream);
+    OSP_LAUNCH_CHECK();
+    return OSP_OK;
+}

@@ -1,0 +1,206 @@
+// Shared by the translation units of attention over documents (attention_packed_fwd.hip, attention_packed_bwd.hip, attention_packed_token.hip):
+// arguments, operand tiles, the two matrix products and the score function.
+//
+//   x = scale q_i . k_j;   c = cap tanh(x / cap) (cap > 0, else x);   s = c - slope_h |pos_i - j|;   pos_i = keys - queries + i
+//   query i sees the keys j < lim_i:   full: all;   causal: lim_i = max(pos_i + 1, prefix)   (a causal and a prefix mask are one limit)
+//   o_i = sum_j softmax_j(s) v_j over the seen keys, 0 where none is seen;  query head h reads key head h / (Hq / Hk)
+//
+// Scores are kept in units of log2 (everything is multiplied by log2 e), so that a probability is one v_exp_f32.
+//
+// Matrix layouts, 32 x 32 tiles (l31 = lane & 31, half = lane >> 5): an A operand holds row l31, a B operand column l31; accumulator element i of a
+// lane is row (i >> 2) * 8 + 4 half + (i & 3), column l31.  bf16: k = 16 a step, a lane holds k = 8 half .. + 7 (v_mfma_f32_32x32x16_bf16);
+// f32: k = 2 a step, a lane holds k = half (v_mfma_f32_32x32x2_f32).
+//   score product  X (32 rows x 32 columns) = R C^T: R's rows from LDS (A), C's rows in registers (B): a lane owns one column entity.
+//   value product  Y^T (width x columns) += W^T X: X's accumulators ARE the B operand when the k indices of a step are taken in accumulator
+//     order; W^T (A) is read from W's LDS rows, bf16 with the transposing ds_read_b64_tr_b16.  The result is transposed: a lane still owns its
+//     column entity, so a softmax's rescaling is one factor per lane and needs no exchange.
+#pragma once
+#include "packed_common.h"
+
+namespace pattn {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float EMPTY = 1.0e30f;             // log-sum-exp of a query that sees nothing: exp2(s - EMPTY) = 0
+constexpr float NONE = -1.0e30f;             // running maximum before the first seen key
+
+enum { CAP = 1, SLOPE = 2 };                 // score function of an instantiation
+
+struct Args {
+    const void *q, *k, *v, *o, *dout;
+    int64_t qr, qh, kr, kh, vr, vh, dor, doh;           // row and head strides in elements (o and the gradients: (rows, heads, D) contiguous)
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;                                 // (Hq, Mq): log2-sum-exp, sum_d dO O
+    const int64_t *qbegin, *qlen, *kbegin, *klen;       // per document
+    const PackedTile* tiles;
+    const int* ntiles;
+    const int64_t* prefix;                              // per document or null
+    const float* slopes;                                // per query head or null
+    int64_t Mq;
+    int cap_tiles, Hq, Hk, G, D, causal;
+    float scale, softcap;
+};
+
+template <typename T> struct Op;
+
+template <> struct Op<__bf16> {
+    typedef pk_bf16x8 Frag;
+    static constexpr int EPC = 8;                                        // elements of a 16-byte chunk
+    template <int DP> static constexpr int NF = DP / 16;
+    static __device__ __forceinline__ f32x16 mma(const Frag a, const Frag b, const f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    // X as the B operand of a value product: 2 steps of 16 rows
+    struct Cols { Frag f[2]; };
+    static __device__ __forceinline__ void set(Cols& x, int i, float p) { x.f[i >> 3][i & 7] = (__bf16)p; }   // probabilities enter the matrix pipe as bf16
+    template <int DP> static __device__ __forceinline__ void value(f32x16 (&y)[DP / 32], const Cols& x, const char* w_l, int lane) {
+        constexpr int ROW = DP * 2 + 16;
+        const int half = lane >> 5, r16 = lane & 15, g16 = (lane >> 4) & 1;
+        const char* base = w_l + (4 * half + (r16 >> 2)) * ROW + (16 * g16 + 4 * (r16 & 3)) * 2;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) {
+                union { s16x4 h[2]; Frag f; } u;
+                const char* a = base + 16 * s * ROW + d * 64;
+                u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+                u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 8 * ROW));
+                y[d] = mma(u.f, x.f[s], y[d]);
+            }
+    }
+    template <int DP> static __device__ __forceinline__ f32x16 score(const char* rows_l, const Frag (&c)[DP / 16], int l31, int half) {
+        constexpr int ROW = DP * 2 + 16;
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) acc = mma(*reinterpret_cast<const Frag*>(rows_l + l31 * ROW + (16 * s + 8 * half) * 2), c[s], acc);
+        return acc;
+    }
+};
+
+template <> struct Op<float> {
+    typedef f32x4 Frag;                                                  // 4 steps: k = (8 g + e, 8 g + 4 + e)
+    static constexpr int EPC = 4;
+    template <int DP> static constexpr int NF = DP / 8;
+    static __device__ __forceinline__ f32x16 mma(float a, float b, const f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+    struct Cols { f32x16 f; };
+    static __device__ __forceinline__ void set(Cols& x, int i, float p) { x.f[i] = p; }
+    template <int DP> static __device__ __forceinline__ void value(f32x16 (&y)[DP / 32], const Cols& x, const char* w_l, int lane) {
+        constexpr int ROW = DP * 4 + 16;
+        const int half = lane >> 5, l31 = lane & 31;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+                y[d] = mma(*reinterpret_cast<const float*>(w_l + ((i >> 2) * 8 + 4 * half + (i & 3)) * ROW + (d * 32 + l31) * 4), x.f[i], y[d]);
+    }
+    template <int DP> static __device__ __forceinline__ f32x16 score(const char* rows_l, const Frag (&c)[DP / 8], int l31, int half) {
+        constexpr int ROW = DP * 4 + 16;
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int g = 0; g < DP / 8; ++g) {
+            const Frag r = *reinterpret_cast<const Frag*>(rows_l + l31 * ROW + (8 * g + 4 * half) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = mma(r[e], c[g][e], acc);
+        }
+        return acc;
+    }
+};
+
+// register fragments (B operand of a score product) of one row; channels from D on are zeros
+template <typename T, int DP>
+__device__ __forceinline__ void load_frags(typename Op<T>::Frag (&f)[Op<T>::template NF<DP>], const T* row, bool valid, int D, int half) {
+    typedef typename Op<T>::Frag Frag;
+    constexpr int E = Op<T>::EPC;
+#pragma unroll
+    for (int s = 0; s < Op<T>::template NF<DP>; ++s) {
+        const int d = (2 * s + half) * E;
+        Frag x = {};
+        if (valid && d < D) x = *reinterpret_cast<const Frag*>(row + d);
+        f[s] = x;
+    }
+}
+
+// R rows of one head -> LDS in two halves: request into registers, store later.  Row stride in LDS: DP elements and 16 bytes (a shift of four banks
+// from row to row).  Rows from nvalid on and channels from D on are zeros: what lies behind a document never enters a product.
+template <typename T, int DP, int R, int NT>
+struct Stage {
+    static constexpr int E = Op<T>::EPC, CPR = DP / E, CHUNKS = R * CPR, N = (CHUNKS + NT - 1) / NT;
+    f32x4 x[N];
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int row0, int nvalid, int D, int tid) {
+#pragma unroll
+        for (int it = 0; it < N; ++it) {
+            const int i = tid + it * NT, r = i / CPR, c = i - r * CPR;
+            x[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if ((CHUNKS % NT == 0 || i < CHUNKS) && row0 + r < nvalid && c * E < D) x[it] = *reinterpret_cast<const f32x4*>(base + (int64_t)(row0 + r) * row_stride + c * E);
+        }
+    }
+    __device__ __forceinline__ void store(char* dst, int tid) const {
+        constexpr int ROW = DP * (int)sizeof(T) + 16;
+#pragma unroll
+        for (int it = 0; it < N; ++it) {
+            const int i = tid + it * NT, r = i / CPR, c = i - r * CPR;
+            if (CHUNKS % NT == 0 || i < CHUNKS) *reinterpret_cast<f32x4*>(dst + r * ROW + c * 16) = x[it];
+        }
+    }
+};
+
+// the values of the same column in both halves of the wave: v_permlane32_swap exchanges the upper half of one register with the lower half of the
+// other.  Written in assembly because the builtin hands back its first result twice here; the waits cover a vector write before and a read behind.
+__device__ __forceinline__ void half_swap(float v, float& lo, float& hi) {
+    lo = v;
+    hi = v;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(lo), "+v"(hi));
+}
+__device__ __forceinline__ float half_max(float v) { float a, b; half_swap(v, a, b); return fmaxf(a, b); }
+__device__ __forceinline__ float half_sum(float v) { float a, b; half_swap(v, a, b); return a + b; }
+
+// The score function of one raw product x = q . k, in log2 units.
+//   EXACT (f32 tensors): tanh by the library;  otherwise 1 - 2 / (exp(2 y) + 1) on v_exp_f32 and v_rcp_f32, off by 2^-23 of the cap at most
+//   slope of the cap, d c / d x = 1 - tanh^2, returned where wanted
+struct Score {
+    float c1, c2, slope2;                 // plain: c1 = scale log2 e;  cap: c1 = 2 scale log2 e / cap (EXACT: scale / cap), c2 = cap log2 e
+    template <int MODE, bool EXACT> __device__ __forceinline__ float value(float x, float distance) const {
+        float s;
+        if constexpr (MODE & CAP) {
+            if constexpr (EXACT) s = c2 * tanhf(x * c1);
+            else s = fmaf(-2.f * c2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f), c2);
+        } else s = x * c1;
+        if constexpr (MODE & SLOPE) s = fmaf(-slope2, fabsf(distance), s);
+        return s;
+    }
+    template <int MODE, bool EXACT> __device__ __forceinline__ float value_and_slope(float x, float distance, float& g) const {
+        float s;
+        g = 1.f;
+        if constexpr (MODE & CAP) {
+            if constexpr (EXACT) { const float t = tanhf(x * c1); s = c2 * t; g = fmaf(-t, t, 1.f); }
+            else { const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f); s = fmaf(-2.f * c2, r, c2); g = 4.f * fmaf(-r, r, r); }
+        } else s = x * c1;
+        if constexpr (MODE & SLOPE) s = fmaf(-slope2, fabsf(distance), s);
+        return s;
+    }
+};
+template <int MODE, bool EXACT> __device__ __forceinline__ Score make_score(const Args& p, int head) {
+    Score s;
+    s.c1 = p.scale * LOG2E; s.c2 = 0.f; s.slope2 = 0.f;
+    if constexpr (MODE & CAP) {
+        s.c1 = EXACT ? p.scale / p.softcap : 2.f * p.scale * LOG2E / p.softcap;
+        s.c2 = p.softcap * LOG2E;
+    }
+    if constexpr (MODE & SLOPE) s.slope2 = p.slopes[head] * LOG2E;
+    return s;
+}
+
+// keys a query at position pos sees
+__device__ __forceinline__ int key_limit(int pos, int klen, int prefix, int causal) {
+    return causal ? min(max(pos + 1, min(prefix, klen)), klen) : klen;
+}
+
+// host: the padded head width an instantiation is made for
+static inline int padded_width(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+
+}  // namespace pattn

@@ -1,0 +1,169 @@
+// Attention over documents, forward: capped scores, a penalty on distance, document, causal and prefix masks, shared key heads.
+// Scores and masks: attention_packed_common.h.  Besides o the kernel keeps one number per query and head, the log2-sum-exp of its scores.
+//
+// One workgroup = 4 waves = one tile of 128 queries of one head; a wave owns 32 queries (one per lane, both halves of the wave hold the same
+// query and half of the keys).  Keys and values pass through LDS in tiles (64 rows, f32: 32), two buffers, one barrier per tile: the next tile's
+// rows are requested into registers before the current tile is computed and stored to the other buffer behind its products.
+//   S^T (keys x queries) = K Q^T;  running maximum and sum per lane;  O^T (width x queries) += V^T P^T
+// The running maximum is moved only when a row's maximum grows by more than 8 (a factor of 256 in the probabilities, which f32 sums and bf16
+// operands carry without loss): the rescaling of O is skipped for nearly every tile after the first.
+#include "attention_packed_common.h"
+
+namespace {
+using namespace pattn;
+
+template <typename T, int DP, int MODE>
+__global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
+    typedef Op<T> O;
+    constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32, ROW = DP * (int)sizeof(T) + 16;
+    constexpr bool EXACT = sizeof(T) == 4;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][KT * ROW];                  // [buffer][K, V]
+    const int h = blockIdx.x % p.Hq, ti = blockIdx.x / p.Hq;
+    if (ti >= p.ntiles[1]) return;
+    const PackedTile tile = p.tiles[ti];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
+    const int w0 = wave * 32, qi = w0 + l31;                                           // this lane's query in the tile
+    const int64_t qrow = (int64_t)tile.row0 + qi;
+    T* out = reinterpret_cast<T*>(p.out) + (qrow * p.Hq + h) * p.D;
+    if (tile.doc < 0) {                                                                // rows of no document
+        if (qi < tile.n)
+            for (int d = half * 8; d < p.D; d += 16)
+                for (int e = 0; e < 8; ++e) out[d + e] = (T)0.f;
+        return;
+    }
+    const int qlen = (int)p.qlen[tile.doc], klen = (int)p.klen[tile.doc];
+    const int prefix = p.prefix ? (int)min(max(p.prefix[tile.doc], (int64_t)0), (int64_t)klen) : 0;
+    const int64_t kb = p.kbegin[tile.doc];
+    const int hk = h / p.G;
+    const T* kp = reinterpret_cast<const T*>(p.k) + kb * p.kr + (int64_t)hk * p.kh;
+    const T* vp = reinterpret_cast<const T*>(p.v) + kb * p.vr + (int64_t)hk * p.vh;
+    const int off = klen - qlen + tile.i0;                                             // position of the tile's first query
+    const int pos = off + qi, lim = qi < tile.n ? key_limit(pos, klen, prefix, p.causal) : 0;
+    const int kmax = max(key_limit(off + tile.n - 1, klen, prefix, p.causal), 0);      // keys any query of the tile sees
+    const int wmax = w0 < tile.n ? max(key_limit(off + min(w0 + 31, tile.n - 1), klen, prefix, p.causal), 0) : 0;   // ... of the wave
+    const int wmin = key_limit(off + w0, klen, prefix, p.causal);                      // keys every query of the wave sees
+    typename O::Frag qf[O::template NF<DP>];
+    load_frags<T, DP>(qf, reinterpret_cast<const T*>(p.q) + qrow * p.qr + (int64_t)h * p.qh, qi < tile.n, p.D, half);
+    const Score sc = make_score<MODE, EXACT>(p, h);
+    f32x16 oacc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) oacc[d][i] = 0.f;
+    float m_run = NONE, l_run = 0.f;
+    const int nt = (kmax + KT - 1) / KT;
+    Stage<T, DP, KT, 256> ks, vs;
+    if (nt > 0) {
+        ks.load(kp, p.kr, 0, klen, p.D, tid);
+        vs.load(vp, p.vr, 0, klen, p.D, tid);
+        ks.store(lds[0][0], tid);
+        vs.store(lds[0][1], tid);
+        if (nt > 1) { ks.load(kp, p.kr, KT, klen, p.D, tid); vs.load(vp, p.vr, KT, klen, p.D, tid); }
+    }
+    __syncthreads();
+    for (int t = 0; t < nt; ++t) {
+        const int k0 = t * KT;
+        const char *kl = lds[t & 1][0], *vl = lds[t & 1][1];
+        if (k0 < wmax) {
+            f32x16 st[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) st[b] = O::template score<DP>(kl + b * 32 * ROW, qf, l31, half);
+            const float dist = (float)(pos - k0 - 4 * half);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) st[b][i] = sc.template value<MODE, EXACT>(st[b][i], dist - (float)(b * 32 + (i >> 2) * 8 + (i & 3)));
+            if (k0 + KT > wmin) {                                                      // some query of the wave does not see the whole tile
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[b][i] = k0 + b * 32 + (i >> 2) * 8 + 4 * half + (i & 3) < lim ? st[b][i] : -INFINITY;
+            }
+            float mx = st[0][0];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[b][i]);
+            mx = half_max(mx);
+            if (__any(mx > m_run + 8.f)) {
+                const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                l_run *= alpha;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) oacc[d][i] *= alpha;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                typename O::Cols pc;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(st[b][i] - m_run);
+                    l_run += e;
+                    O::set(pc, i, e);
+                }
+                O::template value<DP>(oacc, pc, vl + b * 32 * ROW, lane);
+            }
+        }
+        if (t + 1 < nt) {
+            ks.store(lds[(t + 1) & 1][0], tid);
+            vs.store(lds[(t + 1) & 1][1], tid);
+            if (t + 2 < nt) { ks.load(kp, p.kr, k0 + 2 * KT, klen, p.D, tid); vs.load(vp, p.vr, k0 + 2 * KT, klen, p.D, tid); }
+        }
+        __syncthreads();
+    }
+    const float total = half_sum(l_run), inv = total > 0.f ? 1.f / total : 0.f;        // nothing seen: zeros
+    if (qi >= tile.n) return;
+    if (p.lse && half == 0) p.lse[(int64_t)h * p.Mq + qrow] = total > 0.f ? m_run + __log2f(total) : EMPTY;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = d * 32 + g * 8 + 4 * half;
+            const float r[4] = {oacc[d][4 * g] * inv, oacc[d][4 * g + 1] * inv, oacc[d][4 * g + 2] * inv, oacc[d][4 * g + 3] * inv};
+            if (c < p.D) PackedVec<T, 4>::store(out + c, r);
+        }
+}
+
+template <typename T, int DP>
+void launch(const Args& p, hipStream_t s) {
+    const dim3 grid((unsigned)(p.cap_tiles * p.Hq));
+    const int mode = (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0);
+#define L(M_) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, M_>), grid, dim3(256), 0, s, p)
+    if (mode == 0) L(0); else if (mode == 1) L(1); else if (mode == 2) L(2); else L(3);
+#undef L
+}
+template <typename T>
+void launch_width(const Args& p, hipStream_t s) {
+    switch (padded_width(p.D)) {
+        case 32: launch<T, 32>(p, s); break;
+        case 64: launch<T, 64>(p, s); break;
+        case 96: launch<T, 96>(p, s); break;
+        default: launch<T, 128>(p, s);
+    }
+}
+}  // namespace
+
+extern "C" int osp_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                                        int64_t v_row, int64_t v_head, int64_t bf16, void* o, float* lse, const int64_t* qlen, const int32_t* qtiles,
+                                        const int32_t* qntiles, int64_t qcap, const int64_t* kbegin, const int64_t* klen, const int64_t* prefix,
+                                        const float* slopes, int64_t Mq, int64_t Hq, int64_t Hk, int64_t D, float scale, float softcap, int64_t causal,
+                                        hipStream_t stream) {
+    OSP_CHECK_ARG(q && k && v && o && qlen && qtiles && qntiles && kbegin && klen, "null pointer");
+    OSP_CHECK_ARG(Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq <= 65536, "query heads must be a multiple of the key heads");
+    OSP_CHECK_ARG(D > 0 && D <= 128 && D % 8 == 0, "head width must be a multiple of 8, at most 128");
+    const int E = bf16 ? 8 : 4;
+    OSP_CHECK_ARG(q_row % E == 0 && q_head % E == 0 && k_row % E == 0 && k_head % E == 0 && v_row % E == 0 && v_head % E == 0 && packed_aligned(q, 16) &&
+                  packed_aligned(k, 16) && packed_aligned(v, 16) && packed_aligned(o, 16), "rows and heads must start on 16 bytes");
+    OSP_CHECK_ARG(qcap > 0 && qcap * Hq < (int64_t)1 << 31 && softcap >= 0.f && (causal || !prefix), "bad tile list, cap or mask");
+    Args p = {};
+    p.q = q; p.k = k; p.v = v; p.out = o; p.lse = lse;
+    p.qr = q_row; p.qh = q_head; p.kr = k_row; p.kh = k_head; p.vr = v_row; p.vh = v_head;
+    p.qlen = qlen; p.kbegin = kbegin; p.klen = klen; p.tiles = reinterpret_cast<const PackedTile*>(qtiles); p.ntiles = qntiles;
+    p.prefix = prefix; p.slopes = slopes; p.Mq = Mq; p.cap_tiles = (int)qcap; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk); p.D = (int)D;
+    p.causal = (int)(causal != 0); p.scale = scale; p.softcap = softcap;
+    if (bf16) launch_width<__bf16>(p, stream); else launch_width<float>(p, stream);
+    OSP_LAUNCH_CHECK();
+    return OSP_OK;
+}

@@ -217,3 +217,97 @@ def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
                 f"{name} must be a contiguous ({C},) float32 tensor on x's device")
     rows._check(x, "x")
     return GroupNormFn.apply(x, weight, bias, int(groups), rows, float(eps), ACTS[act])
+
+
+# ------------------------------------------------------------------------------------------------------------------ attention over documents
+def _aligned(t, name):
+    """(M, heads, width) whose rows and heads start on 16 bytes (the kernels' access): a copy where they do not."""
+    t = _heads(t, name)
+    e = 16 // t.element_size()
+    return t if t.stride(0) % e == 0 and t.stride(1) % e == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+@_grad_aware
+class PackedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, rows, keys, causal, prefix, softcap, slopes, scale):
+        q, k, v = _aligned(q, "q"), _aligned(k, "k"), _aligned(v, "v")
+        (M, H, D), S = q.shape, k.shape[1]
+        save = _saving(ctx)
+        o = torch.empty((M, H, D), device=q.device, dtype=q.dtype)
+        lse = None
+        if M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536:
+            # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip)
+            ws = _workspace(_size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D), q.device)
+            call("osp_packed_attention_token", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1),
+                 int(q.dtype == torch.bfloat16), o, ws, rows.begin, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length,
+                 keys.longest, prefix, slopes, rows.docs, M, H, S, D, scale, softcap, int(causal))
+        elif M:
+            lse = torch.empty((H, M), device=q.device, dtype=torch.float32) if save else None
+            call("osp_packed_attention_fwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1),
+                 int(q.dtype == torch.bfloat16), o, lse, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, prefix, slopes,
+                 M, H, S, D, scale, softcap, int(causal))
+        if save:
+            ctx.save_for_backward(q, k, v, o, lse, prefix, slopes)
+            ctx.cfg = (rows, keys, causal, softcap, scale)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse, prefix, slopes = ctx.saved_tensors
+        rows, keys, causal, softcap, scale = ctx.cfg
+        (M, H, D), (Mk, S, _) = q.shape, k.shape
+        do = _aligned(do, "the gradient of o")
+        dq = torch.empty((M, H, D), device=q.device, dtype=q.dtype)
+        dk, dv = (torch.empty((Mk, S, D), device=q.device, dtype=q.dtype) for _ in range(2))
+        if M and Mk:
+            delta = torch.empty_like(lse)
+            call("osp_packed_attention_bwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), o, lse, do,
+                 do.stride(0), do.stride(1), int(q.dtype == torch.bfloat16), dq, dk, dv, delta, rows.begin, rows.length, rows.tiles, rows.ntiles,
+                 rows.cap, keys.begin, keys.length, keys.tiles, keys.ntiles, keys.cap, prefix, slopes, M, H, S, D, scale, softcap, int(causal))
+        else:
+            dq.zero_(), dk.zero_(), dv.zero_()
+        return dq, dk, dv, None, None, None, None, None, None, None
+
+
+def attention(q, k, v, rows, keys=None, causal=False, prefix=None, softcap=0.0, slopes=None, scale=None):
+    """softmax(score) v inside each document.  q (M, heads, width), k and v (keys, shared, width) float32 or bfloat16, any row and head strides;
+    width a multiple of 8 up to 128; query head h reads key head h // (heads / shared).
+
+    ``rows`` (PackedRows) lays out the queries; ``keys`` the keys where they differ (a cache: ``PackedRows.from_padded(lengths, capacity)``), with the
+    same number of documents.  Query i of a document stands at position  keys - queries + i : the last query is at the last key.
+
+    score = c(scale q . k) - slopes[head] |position - j|, with c(x) = softcap tanh(x / softcap) where softcap > 0; scale 1 / sqrt(width) unless given;
+    slopes (heads,) float32 (no gradient).  ``causal``: key j is seen from position j on; ``prefix`` (docs,) int64 with it: the first prefix keys of
+    a document are seen by all its queries.  A query that sees nothing gives zeros, and so do rows of no document; gradients likewise.
+    Keys and values must be finite where any query sees them; what lies behind a document is never read into a product.
+
+    float32 tensors are computed in exact 32-bit products, unless the package runs in its bf16 mode: then the operands are rounded to bf16, as in
+    its other attention paths, and the result is float32.  Gradients for q, k and v; no attention dropout."""
+    _refuse(q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2],
+            f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} must be (rows, heads, width), k and v alike")
+    H, S, D = q.shape[1], k.shape[1], q.shape[2]
+    _refuse(S < 1 or H < 1 or H % S or H > 65536, f"{H} query heads do not share {S} key heads evenly")
+    _refuse(D < 8 or D > 128 or D % 8, f"head width {D}: a multiple of 8 up to 128")
+    _refuse(not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.float32, torch.bfloat16),
+            f"q, k, v must be all float32 or all bfloat16, not {q.dtype}, {k.dtype}, {v.dtype}")
+    _refuse(not q.is_cuda or k.device != q.device or v.device != q.device, "q, k, v must live on one GPU")
+    _refuse(prefix is not None and not causal, "a prefix extends a causal mask: pass causal=True with it")
+    _refuse(not softcap >= 0.0 or math.isinf(softcap), f"softcap {softcap}: positive, or 0 for none")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _refuse(not math.isfinite(scale), f"scale {scale}")
+    keys = rows if keys is None else keys
+    rows._check(q, "q")
+    keys._check(k, "k")
+    _refuse(keys.docs != rows.docs, f"{rows.docs} documents of queries, {keys.docs} of keys")
+    if prefix is not None:
+        _refuse(prefix.dtype != torch.int64 or prefix.shape != (rows.docs,) or not prefix.is_contiguous() or prefix.device != q.device,
+                "prefix must be a contiguous (docs,) int64 tensor on q's device")
+    if slopes is not None:
+        _refuse(slopes.dtype != torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous() or slopes.device != q.device,
+                "slopes must be a contiguous (heads,) float32 tensor on q's device")
+        _refuse(slopes.requires_grad, "slopes get no gradient: detach them")
+    if q.dtype == torch.float32 and _precision.is_bf16():
+        q, k, v = q.to(torch.bfloat16), k.to(torch.bfloat16), v.to(torch.bfloat16)
+        return PackedAttentionFn.apply(q, k, v, rows, keys, bool(causal), prefix, float(softcap), slopes, scale).to(torch.float32)
+    return PackedAttentionFn.apply(q, k, v, rows, keys, bool(causal), prefix, float(softcap), slopes, scale)

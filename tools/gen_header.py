@@ -145,6 +145,12 @@ REPLACES = {
     "osp_group_norm_fwd": "no reference counterpart: group norm + activation over the rows of each document (the place of BatchNorm + swish in "
                           "_conformer/convolution.py:61-70, which counts padded frames)",
     "osp_group_norm_bwd": "autograd of the same",
+    "osp_packed_attention_fwd": "MultiHeadedAttention.forward_attention on packed documents, with capped scores, a penalty on distance, causal and prefix "
+                                "masks, shared key heads and different query / key counts (generator/modules/_transformer/attention.py:75-125 "
+                                "knows a key-padding mask)",
+    "osp_packed_attention_bwd": "autograd of the same: probabilities recomputed per tile from q, k and the log-sum-exp",
+    "osp_packed_attention_token_workspace_bytes": "workspace query for osp_packed_attention_token",
+    "osp_packed_attention_token": "osp_packed_attention_fwd for few queries over many keys (new frames over a cache): keys split over workgroups and joined",
     "osp_source_hash": "content hash of the sources this library was built from (optispeech_amd/build.py checks it; no reference counterpart)",
 }
 
