@@ -297,10 +297,10 @@ int osp_conv_gemm_f32_split(const float* A, int64_t lda, int64_t M, int64_t T, i
 int64_t osp_group_norm_workspace_bytes(int64_t B, int64_t M, int64_t C, int64_t G, int64_t backward);
 
 /* replaces: no reference counterpart: group norm + activation over the rows of each document (the place of BatchNorm + swish in _conformer/convolution.py:61-70, which counts padded frames) */
-int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, void* y, float* mean, float* rstd, void* workspace, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, float eps, int64_t act, hipStream_t stream);
+int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, void* y, float* stats, void* workspace, const int64_t* begin, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, float eps, int64_t act, hipStream_t stream);
 
 /* replaces: autograd of the same */
-int osp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, const float* mean, const float* rstd, void* dx, float* dw, float* db, void* workspace, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M, int64_t C, int64_t G, int64_t act, hipStream_t stream);
+int osp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, const float* stats, void* dx, float* dw, int64_t add_w, float* db, int64_t add_b, void* workspace, const int64_t* begin, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, int64_t act, hipStream_t stream);
 
 /* ---- loss.hip ---- */
 /* replaces: FastSpeech2Loss.forward generator/loss.py:83-140, DurationPredictorLoss :28-46 */

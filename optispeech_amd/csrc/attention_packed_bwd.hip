@@ -113,15 +113,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_ke
 
 // ------------------------------------------------------------------------------------------------ dK, dV
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(const Args p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_kernel(const Args p) {
     typedef Op<T> O;
     constexpr int QT = 32, ROW = DP * (int)sizeof(T) + 16;
+    constexpr bool VLDS = sizeof(T) == 2;                                               // V's rows stay in LDS, K's in registers
+    __shared__ __attribute__((aligned(16))) char v_l[VLDS ? PACKED_TILE * ROW : 16];
     constexpr bool EXACT = sizeof(T) == 4;
     __shared__ __attribute__((aligned(16))) char lds[2][2][QT * ROW];                  // [buffer][Q, dO]
     __shared__ __attribute__((aligned(16))) float stat[2][2][QT];                      // [buffer][log2-sum-exp, delta]
     const int hk = blockIdx.x % p.Hk, ti = blockIdx.x / p.Hk;
+    const int ndoc = p.ntiles[0];
     if (ti >= p.ntiles[1]) return;
-    const PackedTile tile = p.tiles[ti];
+    // under a causal mask the first keys have the most queries: the list from its other end
+    const PackedTile tile = p.tiles[p.causal && ti < ndoc ? ndoc - 1 - ti : ti];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, half = lane >> 5;
     const int w0 = wave * 32, ki = w0 + l31;
     const int64_t krow = (int64_t)tile.row0 + ki;
@@ -140,9 +144,14 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(const Args p) {
     const int off = klen - qlen;                                                       // position of the document's first query
     // first query that sees a key of the tile: all see the prefix, key j is seen from position j on
     const int first = !p.causal || tile.i0 < prefix ? 0 : max(tile.i0 - off, 0);
-    typename O::Frag kf[O::template NF<DP>], vf[O::template NF<DP>];
+    typename O::Frag kf[O::template NF<DP>], vf[VLDS ? 1 : O::template NF<DP>];
     load_frags<T, DP>(kf, reinterpret_cast<const T*>(p.k) + krow * p.kr + (int64_t)hk * p.kh, on, p.D, half);
-    load_frags<T, DP>(vf, reinterpret_cast<const T*>(p.v) + krow * p.vr + (int64_t)hk * p.vh, on, p.D, half);
+    const T* vrows = reinterpret_cast<const T*>(p.v) + (int64_t)tile.row0 * p.vr + (int64_t)hk * p.vh;
+    if constexpr (VLDS) {
+        Stage<T, DP, PACKED_TILE, 256> vs;
+        vs.load(vrows, p.vr, 0, tile.n, p.D, tid);
+        vs.store(v_l, tid);
+    } else load_frags<T, DP>(vf, vrows + (int64_t)ki * p.vr, on, p.D, half);
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -183,7 +192,9 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(const Args p) {
         const bool seen = !p.causal || tile.i0 + w0 < prefix || pos0 + QT - 1 >= tile.i0 + w0;
         if (w0 < tile.n && seen) {
             const f32x16 sr = O::template score<DP>(ql, kf, l31, half);
-            const f32x16 dp = O::template score<DP>(dl, vf, l31, half);
+            f32x16 dp;
+            if constexpr (VLDS) dp = O::template score_lds<DP>(dl, v_l + w0 * ROW, l31, half);
+            else dp = O::template score<DP>(dl, vf, l31, half);
             const float dist = (float)(pos0 + 4 * half - key);
             const int row_min = key < prefix ? -0x40000000 : key - pos0 - 4 * half;     // rows (4 half taken off) from here on see the key
             const bool masked = p.causal && pos0 < tile.i0 + w0 + 31;

@@ -78,6 +78,19 @@ template <> struct Op<__bf16> {
         for (int s = 0; s < DP / 16; ++s) acc = mma(*reinterpret_cast<const Frag*>(rows_l + l31 * ROW + (16 * s + 8 * half) * 2), c[s], acc);
         return acc;
     }
+    // the same with C's rows in LDS too
+    template <int DP> static __device__ __forceinline__ f32x16 score_lds(const char* rows_l, const char* c_l, int l31, int half) {
+        constexpr int ROW = DP * 2 + 16;
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int at = l31 * ROW + (16 * s + 8 * half) * 2;
+            acc = mma(*reinterpret_cast<const Frag*>(rows_l + at), *reinterpret_cast<const Frag*>(c_l + at), acc);
+        }
+        return acc;
+    }
 };
 
 template <> struct Op<float> {

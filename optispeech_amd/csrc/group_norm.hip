@@ -60,8 +60,9 @@ struct NormArgs {
     float* cpart;                               // backward: (slots, C, 2)
     double* dsum;                               // backward: (B, C, 2) sums of dz, dz xhat
     float* coef;                                // backward: (B, G, 2) mean(gw), mean(gw xhat)
-    float *dw, *db;
-    const int64_t* len;
+    float *dw, *db;                             // added to where add_w / add_b, written otherwise
+    int add_w, add_b;
+    const int64_t *begin, *len;
     const int* base;
     const PackedTile* tiles;
     const int* ntiles;
@@ -329,8 +330,8 @@ __global__ __launch_bounds__(NTH) void gn_bwd_apply_kernel(const NormArgs p) {
         __syncthreads();
         if (sl == 0 && c < p.C) {
             for (int i = 1; i < 4; ++i) { a += red[i][lane].x; b += red[i][lane].y; }
-            if (p.db) p.db[c] += (float)a;
-            if (p.dw) p.dw[c] += (float)b;
+            if (p.db) p.db[c] = (float)a + (p.add_b ? p.db[c] : 0.f);
+            if (p.dw) p.dw[c] = (float)b + (p.add_w ? p.dw[c] : 0.f);
         }
         return;
     }
@@ -409,16 +410,16 @@ extern "C" int64_t osp_group_norm_workspace_bytes(int64_t B, int64_t M, int64_t 
     return slots * C * 8 + B * C * 16 + B * G * 8 + 512;
 }
 
-extern "C" int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, void* y, float* mean, float* rstd,
-                                  void* workspace, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles,
+extern "C" int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, void* y, float* stats,
+                                  void* workspace, const int64_t* begin, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles,
                                   int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, float eps, int64_t act,
                                   hipStream_t stream) {
-    OSP_CHECK_ARG(x && w && b && y && mean && rstd && workspace && len && base && tiles && ntiles, "null pointer");
+    OSP_CHECK_ARG(x && w && b && y && stats && workspace && begin && len && base && tiles && ntiles, "null pointer");
     OSP_CHECK_ARG(B > 0 && M > 0 && longest > 0 && C > 0 && C <= MAXC && G > 0 && C % G == 0 && ldx >= C, "channels (at most 2048) must be a multiple of groups");
     OSP_CHECK_ARG(eps > 0.f && act >= ACT_NONE && act <= ACT_SILU && cap > 0 && cap < (int64_t)1 << 30 && packed_aligned(workspace, 16), "bad eps, activation or workspace");
     NormArgs p = {};
-    p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.out = y; p.mean = mean; p.rstd = rstd; p.part = reinterpret_cast<double*>(workspace);
-    p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
+    p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.out = y; p.mean = stats; p.rstd = stats + B * G; p.part = reinterpret_cast<double*>(workspace);
+    p.begin = begin; p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
     p.B = (int)B; p.C = (int)C; p.G = (int)G; p.cap = (int)cap; p.sub = parts(M); p.eps = eps;
     const int V = bf16 ? 8 : 4;
     const bool wide = C % V == 0 && ldx % V == 0 && packed_aligned(x, 16) && packed_aligned(y, 16);
@@ -429,16 +430,16 @@ extern "C" int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, cons
 }
 
 extern "C" int osp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b,
-                                  const float* mean, const float* rstd, void* dx, float* dw, float* db, void* workspace, const int64_t* len,
-                                  const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M,
-                                  int64_t C, int64_t G, int64_t act, hipStream_t stream) {
-    OSP_CHECK_ARG(dy && x && w && b && mean && rstd && workspace && len && base && tiles && ntiles, "null pointer");
-    OSP_CHECK_ARG(B > 0 && M > 0 && C > 0 && C <= MAXC && G > 0 && C % G == 0 && ldx >= C && lddy >= C, "channels (at most 2048) must be a multiple of groups");
+                                  const float* stats, void* dx, float* dw, int64_t add_w, float* db, int64_t add_b, void* workspace,
+                                  const int64_t* begin, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles,
+                                  int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, int64_t act, hipStream_t stream) {
+    OSP_CHECK_ARG(dy && x && w && b && stats && workspace && begin && len && base && tiles && ntiles, "null pointer");
+    OSP_CHECK_ARG(B > 0 && M > 0 && longest > 0 && C > 0 && C <= MAXC && G > 0 && C % G == 0 && ldx >= C && lddy >= C, "channels (at most 2048) must be a multiple of groups");
     OSP_CHECK_ARG(act >= ACT_NONE && act <= ACT_SILU && cap > 0 && cap < (int64_t)1 << 30 && packed_aligned(workspace, 16), "bad activation or workspace");
     NormArgs p = {};
     p.x = x; p.ldx = ldx; p.dy = dy; p.lddy = lddy; p.w = w; p.b = b; p.out = dx;
-    p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd); p.dw = dw; p.db = db;
-    p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
+    p.mean = const_cast<float*>(stats); p.rstd = p.mean + B * G; p.dw = dw; p.db = db; p.add_w = (int)(add_w != 0); p.add_b = (int)(add_b != 0);
+    p.begin = begin; p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
     p.B = (int)B; p.C = (int)C; p.G = (int)G; p.cap = (int)cap; p.sub = parts(M);
     const int64_t slots = (M / PACKED_TILE + B) * p.sub;
     char* ws = reinterpret_cast<char*>(workspace);

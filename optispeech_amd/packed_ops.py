@@ -10,26 +10,29 @@ Like the rest of the package: kernels go to torch's current stream on the curren
 ``param.grad`` by the kernels, activations flow through autograd.
 """
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import precision as _precision
 from ._lib import OspError, call, lib
-from .ops import _grad_aware, _saving, _want, gsink
+from .ops import _want
 
 ACTS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 
 
-def _refuse(cond, msg):
-    if cond:
-        raise OspError(msg)
-
-
+@functools.lru_cache(maxsize=4096)
 def _size(name, *args):
+    """a size query of the library: a pure function of its sizes"""
     f = getattr(lib().cdll, name)
     f.restype = ctypes.c_int64
     return f(*(ctypes.c_int64(int(a)) for a in args))
+
+
+def _wants_grad(*ts):
+    """True where autograd records: elsewhere the kernels are called without an autograd node around them"""
+    return torch.is_grad_enabled() and not torch.is_inference_mode_enabled() and any(t.requires_grad for t in ts)
 
 
 class PackedRows:
@@ -37,9 +40,12 @@ class PackedRows:
     host's upper bound ``longest`` on a document's length."""
 
     def __init__(self, src, padded, docs, rows, longest):
-        _refuse(src.dtype != torch.int64 or src.dim() != 1 or not src.is_contiguous(), "offsets / lengths must be a contiguous 1-D int64 tensor")
-        _refuse(not src.is_cuda, "offsets / lengths must live on the GPU")
-        _refuse(docs < 1 or rows < 0 or longest < 0, f"a batch needs at least one document (docs {docs}, rows {rows}, longest {longest})")
+        if src.dtype != torch.int64 or src.dim() != 1 or not src.is_contiguous():
+            raise OspError("offsets / lengths must be a contiguous 1-D int64 tensor")
+        if not src.is_cuda:
+            raise OspError("offsets / lengths must live on the GPU")
+        if docs < 1 or rows < 0 or longest < 0:
+            raise OspError(f"a batch needs at least one document (docs {docs}, rows {rows}, longest {longest})")
         self.docs, self.rows, self.longest, self.device = docs, rows, min(longest, rows), src.device
         self.cap = _size("osp_packed_rows_tiles", docs, rows)
         long = torch.empty((2, docs), device=src.device, dtype=torch.int64)
@@ -62,8 +68,10 @@ class PackedRows:
         return cls(lengths, True, lengths.numel(), lengths.numel() * int(T), int(T))
 
     def _check(self, t, name):
-        _refuse(t.shape[0] != self.rows, f"{name} has {t.shape[0]} rows, the documents were laid out for {self.rows}")
-        _refuse(t.device != self.device, f"{name} is on {t.device}, the documents on {self.device}")
+        if t.shape[0] != self.rows:
+            raise OspError(f"{name} has {t.shape[0]} rows, the documents were laid out for {self.rows}")
+        if t.device != self.device:
+            raise OspError(f"{name} is on {t.device}, the documents on {self.device}")
 
 
 # ------------------------------------------------------------------------------------------------------------------ rotary positions
@@ -77,13 +85,20 @@ class Rotary:
 
     def __init__(self, channels, base=10000.0, layout="half", scaling="none", factor=1.0, original_length=None, slow=1.0, fast=32.0,
                  device="cuda"):
-        _refuse(channels < 2 or channels % 2, f"an even number of channels turns, not {channels}")
-        _refuse(layout not in ("half", "interleaved"), f"layout {layout!r}: 'half' or 'interleaved'")
-        _refuse(scaling not in ("none", "linear", "base", "parts"), f"scaling {scaling!r}: 'none', 'linear', 'base' or 'parts'")
-        _refuse(scaling != "none" and not factor >= 1.0, f"a context is stretched by a factor >= 1, not {factor}")
-        _refuse(scaling == "base" and channels == 2, "a single pair has no slower one for the base to act on")
-        _refuse(scaling == "parts" and (original_length is None or not fast > slow), "scaling 'parts' needs original_length and fast > slow")
-        _refuse(not base > 0.0, f"base {base}")
+        if channels < 2 or channels % 2:
+            raise OspError(f"an even number of channels turns, not {channels}")
+        if layout not in ("half", "interleaved"):
+            raise OspError(f"layout {layout!r}: 'half' or 'interleaved'")
+        if scaling not in ("none", "linear", "base", "parts"):
+            raise OspError(f"scaling {scaling!r}: 'none', 'linear', 'base' or 'parts'")
+        if scaling != "none" and not factor >= 1.0:
+            raise OspError(f"a context is stretched by a factor >= 1, not {factor}")
+        if scaling == "base" and channels == 2:
+            raise OspError("a single pair has no slower one for the base to act on")
+        if scaling == "parts" and (original_length is None or not fast > slow):
+            raise OspError("scaling 'parts' needs original_length and fast > slow")
+        if not base > 0.0:
+            raise OspError(f"base {base}")
         self.channels, self.layout, self.magnitude = int(channels), layout, 1.0
         if scaling == "base":
             base = base * factor ** (channels / (channels - 2))
@@ -102,9 +117,12 @@ class Rotary:
 
 def _heads(t, name):
     """(M, heads, width) with contiguous channels; any row and head stride."""
-    _refuse(t.dim() != 3, f"{name} must be (rows, heads, width), not {tuple(t.shape)}")
-    _refuse(t.dtype not in (torch.float32, torch.bfloat16), f"{name}: float32 or bfloat16, not {t.dtype}")
-    _refuse(not t.is_cuda, f"{name} must live on the GPU")
+    if t.dim() != 3:
+        raise OspError(f"{name} must be (rows, heads, width), not {tuple(t.shape)}")
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise OspError(f"{name}: float32 or bfloat16, not {t.dtype}")
+    if not t.is_cuda:
+        raise OspError(f"{name} must live on the GPU")
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
@@ -140,25 +158,33 @@ def rotary(q, k, rope, rows, first=None, out_dtype=None):
     """Turn the first ``rope.channels`` channels of every head of q (M, heads, width) and k (M, shared, width) by the row's position: its index in
     its document plus ``first`` (docs,) int64 (the frames already in a cache).  One launch; results are contiguous, in ``out_dtype`` (float32
     or bfloat16; the inputs' type without it).  The gradient is the inverse turn, in the inputs' type."""
-    _refuse(q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] < 1 or k.shape[1] < 1,
-            f"q {tuple(q.shape)} and k {tuple(k.shape)} must be (rows, heads, width) with the same rows and width")
-    _refuse(q.dtype != k.dtype, f"q is {q.dtype}, k {k.dtype}")
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] < 1 or k.shape[1] < 1:
+        raise OspError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must be (rows, heads, width) with the same rows and width")
+    if q.dtype != k.dtype:
+        raise OspError(f"q is {q.dtype}, k {k.dtype}")
     out_dtype = q.dtype if out_dtype is None else out_dtype
-    _refuse(out_dtype not in (torch.float32, torch.bfloat16), f"out_dtype: float32 or bfloat16, not {out_dtype}")
-    _refuse(rope.channels > q.shape[2], f"{rope.channels} turned channels in heads of {q.shape[2]}")
-    _refuse(rope.turns.device != q.device, f"the frequencies are on {rope.turns.device}, q on {q.device}")
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise OspError(f"out_dtype: float32 or bfloat16, not {out_dtype}")
+    if rope.channels > q.shape[2]:
+        raise OspError(f"{rope.channels} turned channels in heads of {q.shape[2]}")
+    if rope.turns.device != q.device:
+        raise OspError(f"the frequencies are on {rope.turns.device}, q on {q.device}")
     rows._check(q, "q")
     rows._check(k, "k")
     if first is not None:
-        _refuse(first.dtype != torch.int64 or first.shape != (rows.docs,) or not first.is_contiguous() or first.device != q.device,
-                "first must be a contiguous (docs,) int64 tensor on q's device")
+        if first.dtype != torch.int64 or first.shape != (rows.docs,) or not first.is_contiguous() or first.device != q.device:
+            raise OspError("first must be a contiguous (docs,) int64 tensor on q's device")
+    if not _wants_grad(q, k):
+        return _rotate(q, k, rope, rows, first, out_dtype, False)
     return RotaryFn.apply(q, k, rope, rows, first, out_dtype)
 
 
 # ------------------------------------------------------------------------------------------------------------------ group norm
 def _matrix(t, name):
-    _refuse(t.dim() != 2, f"{name} must be (rows, channels), not {tuple(t.shape)}")
-    _refuse(t.dtype not in (torch.float32, torch.bfloat16), f"{name}: float32 or bfloat16, not {t.dtype}")
+    if t.dim() != 2:
+        raise OspError(f"{name} must be (rows, channels), not {tuple(t.shape)}")
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise OspError(f"{name}: float32 or bfloat16, not {t.dtype}")
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
@@ -167,23 +193,37 @@ def _workspace(nbytes, device):
     return torch.empty((nbytes,), device=device, dtype=torch.uint8)
 
 
-@_grad_aware
+def _normalise(x, w, b, groups, rows, eps, act):
+    """-> (x as the kernel read it, y, mean and rstd)"""
+    x = _matrix(x, "x")
+    M, C = x.shape
+    y = torch.empty((M, C), device=x.device, dtype=x.dtype)
+    stats = torch.empty((2, rows.docs, groups), device=x.device, dtype=torch.float32)
+    if M and rows.longest:
+        ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 0), x.device)
+        call("osp_group_norm_fwd", x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, y, stats, ws, rows.begin, rows.length, rows.base, rows.tiles,
+             rows.ntiles, rows.cap, rows.docs, M, rows.longest, C, groups, eps, act)
+    else:
+        y.zero_()
+    return x, y, stats
+
+
+def _grad_target(p):
+    """(param.grad, 1 where the kernel adds to it, 0 where it was made just now and is written)"""
+    if not _want(p):
+        return None, 0
+    if p.grad is None:
+        p.grad = torch.empty_like(p)
+        return p.grad, 0
+    return p.grad, 1
+
+
 class GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, groups, rows, eps, act):
-        M, C = x.shape
-        x = _matrix(x, "x")
-        y = torch.empty((M, C), device=x.device, dtype=x.dtype)
-        stats = torch.empty((2, rows.docs, groups), device=x.device, dtype=torch.float32)
-        if M and rows.longest:
-            ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 0), x.device)
-            call("osp_group_norm_fwd", x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, y, stats[0], stats[1], ws, rows.length, rows.base,
-                 rows.tiles, rows.ntiles, rows.cap, rows.docs, M, rows.longest, C, groups, float(eps), act)
-        else:
-            y.zero_()
-        if _saving(ctx):
-            ctx.save_for_backward(x, stats)
-            ctx.params, ctx.cfg = (w, b), (groups, rows, act)
+        x, y, stats = _normalise(x, w, b, groups, rows, eps, act)
+        ctx.save_for_backward(x, stats)
+        ctx.params, ctx.cfg = (w, b), (groups, rows, act)
         return y
 
     @staticmethod
@@ -193,29 +233,38 @@ class GroupNormFn(torch.autograd.Function):
         M, C = x.shape
         dy = _matrix(dy, "dy")
         dx = torch.empty((M, C), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
+        (dw, add_w), (db, add_b) = _grad_target(w), _grad_target(b)
         if M and rows.longest:
             ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 1), x.device)
-            call("osp_group_norm_bwd", dy, dy.stride(0), x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, stats[0], stats[1], dx,
-                 gsink(w) if _want(w) else None, gsink(b) if _want(b) else None, ws, rows.length, rows.base, rows.tiles, rows.ntiles, rows.cap,
-                 rows.docs, M, C, groups, act)
-        elif dx is not None:
-            dx.zero_()
+            call("osp_group_norm_bwd", dy, dy.stride(0), x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, stats, dx, dw, add_w, db, add_b, ws,
+                 rows.begin, rows.length, rows.base, rows.tiles, rows.ntiles, rows.cap, rows.docs, M, rows.longest, C, groups, act)
+        else:
+            for t, add in ((dx, 0), (dw, add_w), (db, add_b)):
+                if t is not None and not add:
+                    t.zero_()
         return dx, None, None, None, None, None, None
 
 
 def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
     """act(weight * (x - mean) / sqrt(var + eps) + bias), mean and variance over a document's rows and a group's channels.  x (M, C) float32
     or bfloat16 (any row stride), weight / bias (C,) float32, act None, "relu", "gelu" (with erf) or "silu"; C <= 2048."""
-    _refuse(x.dim() != 2 or not x.is_cuda, "x must be a (rows, channels) tensor on the GPU")
-    _refuse(x.dtype not in (torch.float32, torch.bfloat16), f"x: float32 or bfloat16, not {x.dtype}")
+    if x.dim() != 2 or not x.is_cuda:
+        raise OspError("x must be a (rows, channels) tensor on the GPU")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise OspError(f"x: float32 or bfloat16, not {x.dtype}")
     C = x.shape[1]
-    _refuse(groups < 1 or C < 1 or C % groups or C > 2048, f"{C} channels (at most 2048) do not divide into {groups} groups")
-    _refuse(act not in ACTS, f"act {act!r}: one of {sorted(a for a in ACTS if a)} or None")
-    _refuse(not eps > 0.0, f"eps {eps}")
+    if groups < 1 or C < 1 or C % groups or C > 2048:
+        raise OspError(f"{C} channels (at most 2048) do not divide into {groups} groups")
+    if act not in ACTS:
+        raise OspError(f"act {act!r}: one of {sorted(a for a in ACTS if a)} or None")
+    if not eps > 0.0:
+        raise OspError(f"eps {eps}")
     for name, t in (("weight", weight), ("bias", bias)):
-        _refuse(t.shape != (C,) or t.dtype != torch.float32 or not t.is_contiguous() or t.device != x.device,
-                f"{name} must be a contiguous ({C},) float32 tensor on x's device")
+        if t.shape != (C,) or t.dtype != torch.float32 or not t.is_contiguous() or t.device != x.device:
+            raise OspError(f"{name} must be a contiguous ({C},) float32 tensor on x's device")
     rows._check(x, "x")
+    if not _wants_grad(x, weight, bias):
+        return _normalise(x, weight, bias, int(groups), rows, float(eps), ACTS[act])[1]
     return GroupNormFn.apply(x, weight, bias, int(groups), rows, float(eps), ACTS[act])
 
 
@@ -227,29 +276,30 @@ def _aligned(t, name):
     return t if t.stride(0) % e == 0 and t.stride(1) % e == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
 
 
-@_grad_aware
+def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):
+    """-> (q, k, v as the kernels read them, o, log2-sum-exp or None)"""
+    q, k, v = _aligned(q, "q"), _aligned(k, "k"), _aligned(v, "v")
+    (M, H, D), S, bf16 = q.shape, k.shape[1], int(q.dtype == torch.bfloat16)
+    o = torch.empty((M, H, D), device=q.device, dtype=q.dtype)
+    lse = torch.empty((H, M), device=q.device, dtype=torch.float32) if save else None
+    if M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536:
+        # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip)
+        ws = _workspace(_size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D), q.device)
+        call("osp_packed_attention_token", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, ws,
+             rows.begin, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, keys.longest, prefix, slopes, rows.docs, M, H, S,
+             D, scale, softcap, causal)
+    elif M:
+        call("osp_packed_attention_fwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, lse,
+             rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, prefix, slopes, M, H, S, D, scale, softcap, causal)
+    return q, k, v, o, lse
+
+
 class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, rows, keys, causal, prefix, softcap, slopes, scale):
-        q, k, v = _aligned(q, "q"), _aligned(k, "k"), _aligned(v, "v")
-        (M, H, D), S = q.shape, k.shape[1]
-        save = _saving(ctx)
-        o = torch.empty((M, H, D), device=q.device, dtype=q.dtype)
-        lse = None
-        if M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536:
-            # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip)
-            ws = _workspace(_size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D), q.device)
-            call("osp_packed_attention_token", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1),
-                 int(q.dtype == torch.bfloat16), o, ws, rows.begin, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length,
-                 keys.longest, prefix, slopes, rows.docs, M, H, S, D, scale, softcap, int(causal))
-        elif M:
-            lse = torch.empty((H, M), device=q.device, dtype=torch.float32) if save else None
-            call("osp_packed_attention_fwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1),
-                 int(q.dtype == torch.bfloat16), o, lse, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, prefix, slopes,
-                 M, H, S, D, scale, softcap, int(causal))
-        if save:
-            ctx.save_for_backward(q, k, v, o, lse, prefix, slopes)
-            ctx.cfg = (rows, keys, causal, softcap, scale)
+        q, k, v, o, lse = _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, prefix, slopes)
+        ctx.cfg = (rows, keys, causal, softcap, scale)
         return o
 
     @staticmethod
@@ -264,7 +314,7 @@ class PackedAttentionFn(torch.autograd.Function):
             delta = torch.empty_like(lse)
             call("osp_packed_attention_bwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), o, lse, do,
                  do.stride(0), do.stride(1), int(q.dtype == torch.bfloat16), dq, dk, dv, delta, rows.begin, rows.length, rows.tiles, rows.ntiles,
-                 rows.cap, keys.begin, keys.length, keys.tiles, keys.ntiles, keys.cap, prefix, slopes, M, H, S, D, scale, softcap, int(causal))
+                 rows.cap, keys.begin, keys.length, keys.tiles, keys.ntiles, keys.cap, prefix, slopes, M, H, S, D, scale, softcap, causal)
         else:
             dq.zero_(), dk.zero_(), dv.zero_()
         return dq, dk, dv, None, None, None, None, None, None, None
@@ -284,30 +334,40 @@ def attention(q, k, v, rows, keys=None, causal=False, prefix=None, softcap=0.0, 
 
     float32 tensors are computed in exact 32-bit products, unless the package runs in its bf16 mode: then the operands are rounded to bf16, as in
     its other attention paths, and the result is float32.  Gradients for q, k and v; no attention dropout."""
-    _refuse(q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2],
-            f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} must be (rows, heads, width), k and v alike")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise OspError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} must be (rows, heads, width), k and v alike")
     H, S, D = q.shape[1], k.shape[1], q.shape[2]
-    _refuse(S < 1 or H < 1 or H % S or H > 65536, f"{H} query heads do not share {S} key heads evenly")
-    _refuse(D < 8 or D > 128 or D % 8, f"head width {D}: a multiple of 8 up to 128")
-    _refuse(not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.float32, torch.bfloat16),
-            f"q, k, v must be all float32 or all bfloat16, not {q.dtype}, {k.dtype}, {v.dtype}")
-    _refuse(not q.is_cuda or k.device != q.device or v.device != q.device, "q, k, v must live on one GPU")
-    _refuse(prefix is not None and not causal, "a prefix extends a causal mask: pass causal=True with it")
-    _refuse(not softcap >= 0.0 or math.isinf(softcap), f"softcap {softcap}: positive, or 0 for none")
+    if S < 1 or H < 1 or H % S or H > 65536:
+        raise OspError(f"{H} query heads do not share {S} key heads evenly")
+    if D < 8 or D > 128 or D % 8:
+        raise OspError(f"head width {D}: a multiple of 8 up to 128")
+    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.float32, torch.bfloat16):
+        raise OspError(f"q, k, v must be all float32 or all bfloat16, not {q.dtype}, {k.dtype}, {v.dtype}")
+    if not q.is_cuda or k.device != q.device or v.device != q.device:
+        raise OspError("q, k, v must live on one GPU")
+    if prefix is not None and not causal:
+        raise OspError("a prefix extends a causal mask: pass causal=True with it")
+    if not softcap >= 0.0 or math.isinf(softcap):
+        raise OspError(f"softcap {softcap}: positive, or 0 for none")
     scale = D ** -0.5 if scale is None else float(scale)
-    _refuse(not math.isfinite(scale), f"scale {scale}")
+    if not math.isfinite(scale):
+        raise OspError(f"scale {scale}")
     keys = rows if keys is None else keys
     rows._check(q, "q")
     keys._check(k, "k")
-    _refuse(keys.docs != rows.docs, f"{rows.docs} documents of queries, {keys.docs} of keys")
+    if keys.docs != rows.docs:
+        raise OspError(f"{rows.docs} documents of queries, {keys.docs} of keys")
     if prefix is not None:
-        _refuse(prefix.dtype != torch.int64 or prefix.shape != (rows.docs,) or not prefix.is_contiguous() or prefix.device != q.device,
-                "prefix must be a contiguous (docs,) int64 tensor on q's device")
+        if prefix.dtype != torch.int64 or prefix.shape != (rows.docs,) or not prefix.is_contiguous() or prefix.device != q.device:
+            raise OspError("prefix must be a contiguous (docs,) int64 tensor on q's device")
     if slopes is not None:
-        _refuse(slopes.dtype != torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous() or slopes.device != q.device,
-                "slopes must be a contiguous (heads,) float32 tensor on q's device")
-        _refuse(slopes.requires_grad, "slopes get no gradient: detach them")
-    if q.dtype == torch.float32 and _precision.is_bf16():
+        if slopes.dtype != torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous() or slopes.device != q.device:
+            raise OspError("slopes must be a contiguous (heads,) float32 tensor on q's device")
+        if slopes.requires_grad:
+            raise OspError("slopes get no gradient: detach them")
+    rounded = q.dtype == torch.float32 and _precision.is_bf16()
+    if rounded:
         q, k, v = q.to(torch.bfloat16), k.to(torch.bfloat16), v.to(torch.bfloat16)
-        return PackedAttentionFn.apply(q, k, v, rows, keys, bool(causal), prefix, float(softcap), slopes, scale).to(torch.float32)
-    return PackedAttentionFn.apply(q, k, v, rows, keys, bool(causal), prefix, float(softcap), slopes, scale)
+    args = (q, k, v, rows, keys, int(bool(causal)), prefix, float(softcap), slopes, scale)
+    o = PackedAttentionFn.apply(*args) if _wants_grad(q, k, v) else _attend(*args, False)[3]
+    return o.to(torch.float32) if rounded else o
