@@ -7,6 +7,7 @@
 //        dK^T += Q^T dS): the sum over shared heads stays in its accumulators
 // S and dP are computed twice, 7 instead of 5 products per tile pair: the price of combining dQ without atomics or a partial dQ per key tile.
 #include "attention_packed_common.h"
+#include <type_traits>
 
 namespace {
 using namespace pattn;
@@ -44,20 +45,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_ke
     const int wmin = key_limit(off + w0, klen, prefix, p.causal);
     const bool on = qi < tile.n;
     typename O::Frag qf[O::template NF<DP>], dof[O::template NF<DP>];
-    load_frags<T, DP>(dof, reinterpret_cast<const T*>(p.dout) + qrow * p.dor + (int64_t)h * p.doh, on, p.D, half);
+    const int64_t row0 = tile.row0, orow = (int64_t)p.Hq * p.D;
+    load_frags<T, DP>(dof, row_buffer(reinterpret_cast<const T*>(p.dout) + row0 * p.dor + (int64_t)h * p.doh, p.dor, tile.n), p.dor, qi, p.D, half);
     float delta = 0.f;
     {
-        load_frags<T, DP>(qf, reinterpret_cast<const T*>(p.o) + (qrow * p.Hq + h) * p.D, on, p.D, half);   // o, then q
+        load_frags<T, DP>(qf, row_buffer(reinterpret_cast<const T*>(p.o) + row0 * orow + h * p.D, orow, tile.n), orow, qi, p.D, half);   // o, then q
 #pragma unroll
         for (int s = 0; s < O::template NF<DP>; ++s)
 #pragma unroll
             for (int e = 0; e < O::EPC; ++e) delta = fmaf((float)dof[s][e], (float)qf[s][e], delta);
+        if constexpr (!EXACT) {                                                         // what o's rounding took off
+            load_frags<T, DP>(qf, row_buffer(reinterpret_cast<const T*>(p.rest) + row0 * orow + h * p.D, orow, tile.n), orow, qi, p.D, half);
+#pragma unroll
+            for (int s = 0; s < O::template NF<DP>; ++s)
+#pragma unroll
+                for (int e = 0; e < O::EPC; ++e) delta = fmaf((float)dof[s][e], (float)qf[s][e], delta);
+        }
         delta = half_sum(delta);
         if (on && half == 0) p.delta[(int64_t)h * p.Mq + qrow] = delta;
     }
-    load_frags<T, DP>(qf, reinterpret_cast<const T*>(p.q) + qrow * p.qr + (int64_t)h * p.qh, on, p.D, half);
-    const float lse = on ? p.lse[(int64_t)h * p.Mq + qrow] : EMPTY;
-    const Score sc = make_score<MODE, EXACT>(p, h);
+    load_frags<T, DP>(qf, row_buffer(reinterpret_cast<const T*>(p.q) + row0 * p.qr + (int64_t)h * p.qh, p.qr, tile.n), p.qr, qi, p.D, half);
+    const Score<MODE, EXACT> sc(p, h);
+    const float shift = sc.fb - (on ? p.lse[(int64_t)h * p.Mq + qrow] : EMPTY), back = p.scale * sc.grad_scale;
     f32x16 acc[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -66,11 +75,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_ke
     const int nt = (kmax + KT - 1) / KT;
     Stage<T, DP, KT, 256> ks, vs;
     if (nt > 0) {
-        ks.load(kp, p.kr, 0, klen, p.D, tid);
-        vs.load(vp, p.vr, 0, klen, p.D, tid);
+        ks.load(kp, p.kr, klen, p.D, tid);
+        vs.load(vp, p.vr, klen, p.D, tid);
         ks.store(lds[0][0], tid);
         vs.store(lds[0][1], tid);
-        if (nt > 1) { ks.load(kp, p.kr, KT, klen, p.D, tid); vs.load(vp, p.vr, KT, klen, p.D, tid); }
+        if (nt > 1) { ks.load(kp + KT * p.kr, p.kr, klen - KT, p.D, tid); vs.load(vp + KT * p.vr, p.vr, klen - KT, p.D, tid); }
     }
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
@@ -78,25 +87,38 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_ke
         const char *kl = lds[t & 1][0], *vl = lds[t & 1][1];
         if (k0 < wmax) {
             const float dist = (float)(pos - k0 - 4 * half);
-            const bool masked = k0 + KT > wmin;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                f32x16 st = O::template score<DP>(kl + b * 32 * ROW, qf, l31, half);
-                const f32x16 dp = O::template score<DP>(vl + b * 32 * ROW, dof, l31, half);
+            const int left = lim - k0 - 4 * half;                                      // rows of the tile this lane's query sees
+            auto block = [&](int b, auto masked) {
+                const char *kt = kl + b * 32 * ROW, *vt = vl + b * 32 * ROW;
+                const f32x16 st = O::template score<DP>(kt, qf, l31, half, splat(0.f));
+                const f32x16 dp = O::template score<DP>(vt, dof, l31, half, splat(-delta));       // dP - delta
+                float at = dist;
+                if constexpr (MODE & SLOPE) asm volatile("" : "+v"(at));              // keeps a whole tile's penalties from being computed ahead of the branch
                 typename O::Cols ds;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float g, s = sc.template value_and_slope<MODE, EXACT>(st[i], dist - (float)(b * 32 + (i >> 2) * 8 + (i & 3)), g);
-                    if (masked) s = k0 + b * 32 + (i >> 2) * 8 + 4 * half + (i & 3) < lim ? s : -INFINITY;
-                    O::set(ds, i, __builtin_amdgcn_exp2f(s - lse) * (dp[i] - delta) * g);
+                    const int r = b * 32 + (i >> 2) * 8 + (i & 3);
+                    const float c = sc.cap(st[i]);
+                    float pr = __builtin_amdgcn_exp2f(fmaf(sc.penalise(c, at - (float)r), sc.fa, shift));
+                    if constexpr (masked) pr = r < left ? pr : 0.f;
+                    float d = dp[i];
+                    if constexpr (MODE & CAP) d *= sc.derive(c);
+                    O::set(ds, i, pr * d);
                 }
-                O::template value<DP>(acc, ds, kl + b * 32 * ROW, lane);
+                O::template value<DP>(acc, ds, kt, lane);
+            };
+            if (k0 + KT > wmin) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) block(b, std::true_type{});
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) block(b, std::false_type{});
             }
         }
         if (t + 1 < nt) {
             ks.store(lds[(t + 1) & 1][0], tid);
             vs.store(lds[(t + 1) & 1][1], tid);
-            if (t + 2 < nt) { ks.load(kp, p.kr, k0 + 2 * KT, klen, p.D, tid); vs.load(vp, p.vr, k0 + 2 * KT, klen, p.D, tid); }
+            if (t + 2 < nt) { ks.load(kp + (int64_t)(k0 + 2 * KT) * p.kr, p.kr, klen - k0 - 2 * KT, p.D, tid); vs.load(vp + (int64_t)(k0 + 2 * KT) * p.vr, p.vr, klen - k0 - 2 * KT, p.D, tid); }
         }
         __syncthreads();
     }
@@ -105,8 +127,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_ke
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int c = d * 32 + g * 8 + 4 * half;
-            const float r[4] = {acc[d][4 * g] * p.scale, acc[d][4 * g + 1] * p.scale, acc[d][4 * g + 2] * p.scale, acc[d][4 * g + 3] * p.scale};
+            const int c = O::template channel<DP>(d, g, half);
+            const float r[4] = {acc[d][4 * g] * back, acc[d][4 * g + 1] * back, acc[d][4 * g + 2] * back, acc[d][4 * g + 3] * back};
             if (c < p.D) PackedVec<T, 4>::store(out + c, r);
         }
 }
@@ -120,7 +142,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_k
     __shared__ __attribute__((aligned(16))) char v_l[VLDS ? PACKED_TILE * ROW : 16];
     constexpr bool EXACT = sizeof(T) == 4;
     __shared__ __attribute__((aligned(16))) char lds[2][2][QT * ROW];                  // [buffer][Q, dO]
-    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];                      // [buffer][log2-sum-exp, delta]
+    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];                      // [buffer][b - log2-sum-exp, -delta]
     const int hk = blockIdx.x % p.Hk, ti = blockIdx.x / p.Hk;
     const int ndoc = p.ntiles[0];
     if (ti >= p.ntiles[1]) return;
@@ -145,13 +167,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_k
     // first query that sees a key of the tile: all see the prefix, key j is seen from position j on
     const int first = !p.causal || tile.i0 < prefix ? 0 : max(tile.i0 - off, 0);
     typename O::Frag kf[O::template NF<DP>], vf[VLDS ? 1 : O::template NF<DP>];
-    load_frags<T, DP>(kf, reinterpret_cast<const T*>(p.k) + krow * p.kr + (int64_t)hk * p.kh, on, p.D, half);
+    load_frags<T, DP>(kf, row_buffer(reinterpret_cast<const T*>(p.k) + (int64_t)tile.row0 * p.kr + (int64_t)hk * p.kh, p.kr, tile.n), p.kr, ki, p.D, half);
     const T* vrows = reinterpret_cast<const T*>(p.v) + (int64_t)tile.row0 * p.vr + (int64_t)hk * p.vh;
     if constexpr (VLDS) {
         Stage<T, DP, PACKED_TILE, 256> vs;
-        vs.load(vrows, p.vr, 0, tile.n, p.D, tid);
+        vs.load(vrows, p.vr, tile.n, p.D, tid);
         vs.store(v_l, tid);
-    } else load_frags<T, DP>(vf, vrows + (int64_t)ki * p.vr, on, p.D, half);
+    } else load_frags<T, DP>(vf, row_buffer(vrows, p.vr, tile.n), p.vr, ki, p.D, half);
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -159,16 +181,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_k
         for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
     const int key = tile.i0 + ki;                                                      // this lane's key in the document
     const int nqt = first < qlen ? (qlen - first + QT - 1) / QT : 0, nt = nqt * p.G;
+    Score<MODE, EXACT> sc(p, hk * p.G);
+    const float back = p.scale * sc.grad_scale;
     Stage<T, DP, QT, 256> qs, dos;
     float st_reg = 0.f;
     auto load = [&](int t) {
         const int h = hk * p.G + t / nqt, r0 = first + (t % nqt) * QT;
-        qs.load(reinterpret_cast<const T*>(p.q) + qb * p.qr + (int64_t)h * p.qh, p.qr, r0, qlen, p.D, tid);
-        dos.load(reinterpret_cast<const T*>(p.dout) + qb * p.dor + (int64_t)h * p.doh, p.dor, r0, qlen, p.D, tid);
+        qs.load(reinterpret_cast<const T*>(p.q) + (qb + r0) * p.qr + (int64_t)h * p.qh, p.qr, qlen - r0, p.D, tid);
+        dos.load(reinterpret_cast<const T*>(p.dout) + (qb + r0) * p.dor + (int64_t)h * p.doh, p.dor, qlen - r0, p.D, tid);
         if (tid < 2 * QT) {
             const int r = r0 + (tid & (QT - 1));
             const float* src = tid < QT ? p.lse : p.delta;
-            st_reg = r < qlen ? src[(int64_t)h * p.Mq + qb + r] : tid < QT ? EMPTY : 0.f;
+            st_reg = (tid < QT ? sc.fb : 0.f) - (r < qlen ? src[(int64_t)h * p.Mq + qb + r] : tid < QT ? EMPTY : 0.f);
         }
     };
     auto store = [&](int buf) {
@@ -182,37 +206,47 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_k
         if (nt > 1) load(1);
     }
     __syncthreads();
-    Score sc = make_score<MODE, EXACT>(p, hk * p.G);
     for (int t = 0; t < nt; ++t) {
         const int buf = t & 1, r0 = first + (t % nqt) * QT;
-        if constexpr (MODE & SLOPE) sc.slope2 = p.slopes[hk * p.G + t / nqt] * LOG2E;
+        sc.set_head(p, hk * p.G + t / nqt);
         const char *ql = lds[buf][0], *dl = lds[buf][1];
         const int pos0 = off + r0;
         // the wave's keys are all behind the tile's last query: nothing seen
         const bool seen = !p.causal || tile.i0 + w0 < prefix || pos0 + QT - 1 >= tile.i0 + w0;
         if (w0 < tile.n && seen) {
-            const f32x16 sr = O::template score<DP>(ql, kf, l31, half);
-            f32x16 dp;
-            if constexpr (VLDS) dp = O::template score_lds<DP>(dl, v_l + w0 * ROW, l31, half);
-            else dp = O::template score<DP>(dl, vf, l31, half);
-            const float dist = (float)(pos0 + 4 * half - key);
-            const int row_min = key < prefix ? -0x40000000 : key - pos0 - 4 * half;     // rows (4 half taken off) from here on see the key
-            const bool masked = p.causal && pos0 < tile.i0 + w0 + 31;
-            typename O::Cols pc, ds;
+            f32x16 dp;                                                                  // starts at -delta of its rows
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
-                const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[buf][0][g4 * 8 + 4 * half]);
                 const f32x4 del = *reinterpret_cast<const f32x4*>(&stat[buf][1][g4 * 8 + 4 * half]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = g4 * 4 + e;
-                    float g, s = sc.template value_and_slope<MODE, EXACT>(sr[i], dist + (float)(g4 * 8 + e), g);
-                    if (masked) s = g4 * 8 + e >= row_min ? s : -INFINITY;
-                    const float pr = __builtin_amdgcn_exp2f(s - lse[e]);
-                    O::set(pc, i, pr);
-                    O::set(ds, i, pr * (dp[i] - del[e]) * g);
-                }
+                for (int e = 0; e < 4; ++e) dp[g4 * 4 + e] = del[e];
             }
+            const f32x16 sr = O::template score<DP>(ql, kf, l31, half, splat(0.f));
+            if constexpr (VLDS) dp = O::template score_lds<DP>(dl, v_l + w0 * ROW, l31, half, dp);
+            else dp = O::template score<DP>(dl, vf, l31, half, dp);
+            const float dist = (float)(pos0 + 4 * half - key);
+            const int row_min = key < prefix ? -0x40000000 : key - pos0 - 4 * half;      // rows (4 half taken off) from here on see the key
+            typename O::Cols pc, ds;
+            auto elements = [&](auto masked) {
+                float at = dist;
+                if constexpr (MODE & SLOPE) asm volatile("" : "+v"(at));
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const f32x4 shift = *reinterpret_cast<const f32x4*>(&stat[buf][0][g4 * 8 + 4 * half]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = g4 * 4 + e, r = g4 * 8 + e;
+                        const float c = sc.cap(sr[i]);
+                        float pr = __builtin_amdgcn_exp2f(fmaf(sc.penalise(c, at + (float)r), sc.fa, shift[e]));
+                        if constexpr (masked) pr = r >= row_min ? pr : 0.f;
+                        float d = dp[i];
+                        if constexpr (MODE & CAP) d *= sc.derive(c);
+                        O::set(pc, i, pr);
+                        O::set(ds, i, pr * d);
+                    }
+                }
+            };
+            if (p.causal && pos0 < tile.i0 + w0 + 31) elements(std::true_type{}); else elements(std::false_type{});
             O::template value<DP>(dv, pc, dl, lane);
             O::template value<DP>(dk, ds, ql, lane);
         }
@@ -227,8 +261,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_k
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int c = d * 32 + g * 8 + 4 * half;
-            const float a[4] = {dk[d][4 * g] * p.scale, dk[d][4 * g + 1] * p.scale, dk[d][4 * g + 2] * p.scale, dk[d][4 * g + 3] * p.scale};
+            const int c = O::template channel<DP>(d, g, half);
+            const float a[4] = {dk[d][4 * g] * back, dk[d][4 * g + 1] * back, dk[d][4 * g + 2] * back, dk[d][4 * g + 3] * back};
             const float b[4] = {dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
             if (c < p.D) { PackedVec<T, 4>::store(outk + c, a); PackedVec<T, 4>::store(outv + c, b); }
         }
@@ -258,13 +292,13 @@ void launch_width(const Args& p, const PackedTile* kt, const int* kn, int kcap, 
 }  // namespace
 
 extern "C" int osp_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
-                                        int64_t v_row, int64_t v_head, const void* o, const float* lse, const void* dout, int64_t do_row,
+                                        int64_t v_row, int64_t v_head, const void* o, const void* rest, const float* lse, const void* dout, int64_t do_row,
                                         int64_t do_head, int64_t bf16, void* dq, void* dk, void* dv, float* delta, const int64_t* qbegin,
                                         const int64_t* qlen, const int32_t* qtiles, const int32_t* qntiles, int64_t qcap, const int64_t* kbegin,
                                         const int64_t* klen, const int32_t* ktiles, const int32_t* kntiles, int64_t kcap, const int64_t* prefix,
                                         const float* slopes, int64_t Mq, int64_t Hq, int64_t Hk, int64_t D, float scale, float softcap, int64_t causal,
                                         hipStream_t stream) {
-    OSP_CHECK_ARG(q && k && v && o && lse && dout && dq && dk && dv && delta && qbegin && qlen && qtiles && qntiles && kbegin && klen && ktiles && kntiles,
+    OSP_CHECK_ARG(q && k && v && o && (rest || !bf16) && lse && dout && dq && dk && dv && delta && qbegin && qlen && qtiles && qntiles && kbegin && klen && ktiles && kntiles,
                   "null pointer");
     OSP_CHECK_ARG(Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq <= 65536, "query heads must be a multiple of the key heads");
     OSP_CHECK_ARG(D > 0 && D <= 128 && D % 8 == 0, "head width must be a multiple of 8, at most 128");
@@ -272,10 +306,11 @@ extern "C" int osp_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_
     OSP_CHECK_ARG(q_row % E == 0 && q_head % E == 0 && k_row % E == 0 && k_head % E == 0 && v_row % E == 0 && v_head % E == 0 && do_row % E == 0 &&
                   do_head % E == 0 && packed_aligned(q, 16) && packed_aligned(k, 16) && packed_aligned(v, 16) && packed_aligned(dout, 16) &&
                   packed_aligned(o, 16) && packed_aligned(dq, 16) && packed_aligned(dk, 16) && packed_aligned(dv, 16), "rows and heads must start on 16 bytes");
-    OSP_CHECK_ARG(qcap > 0 && kcap > 0 && qcap * Hq < (int64_t)1 << 31 && kcap * Hk < (int64_t)1 << 31 && softcap >= 0.f && (causal || !prefix),
+    OSP_CHECK_ARG(qcap > 0 && kcap > 0 && qcap * Hq < (int64_t)1 << 31 && kcap * Hk < (int64_t)1 << 31 && scale > 0.f && softcap >= 0.f && (causal || !prefix),
                   "bad tile list, cap or mask");
+    OSP_CHECK_ARG(row_stride_ok(Hq * D, D, bf16) && row_stride_ok(q_row, D, bf16) && row_stride_ok(k_row, D, bf16) && row_stride_ok(v_row, D, bf16) && row_stride_ok(do_row, D, bf16), "row strides must lie between the head width and 2^24 bytes");
     Args p = {};
-    p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv; p.lse = const_cast<float*>(lse); p.delta = delta;
+    p.q = q; p.k = k; p.v = v; p.o = o; p.rest = const_cast<void*>(rest); p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv; p.lse = const_cast<float*>(lse); p.delta = delta;
     p.qr = q_row; p.qh = q_head; p.kr = k_row; p.kh = k_head; p.vr = v_row; p.vh = v_head; p.dor = do_row; p.doh = do_head;
     p.qbegin = qbegin; p.qlen = qlen; p.kbegin = kbegin; p.klen = klen; p.tiles = reinterpret_cast<const PackedTile*>(qtiles); p.ntiles = qntiles;
     p.prefix = prefix; p.slopes = slopes; p.Mq = Mq; p.cap_tiles = (int)qcap; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk); p.D = (int)D;

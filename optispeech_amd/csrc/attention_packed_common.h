@@ -31,6 +31,7 @@ enum { CAP = 1, SLOPE = 2 };                 // score function of an instantiati
 
 struct Args {
     const void *q, *k, *v, *o, *dout;
+    void* rest;                                         // bf16: o's rounding error, (rows, heads, D), or null
     int64_t qr, qh, kr, kh, vr, vh, dor, doh;           // row and head strides in elements (o and the gradients: (rows, heads, D) contiguous)
     void *out, *dq, *dk, *dv;
     float *lse, *delta;                                 // (Hq, Mq): log2-sum-exp, sum_d dO O
@@ -54,36 +55,34 @@ template <> struct Op<__bf16> {
     // X as the B operand of a value product: 2 steps of 16 rows
     struct Cols { Frag f[2]; };
     static __device__ __forceinline__ void set(Cols& x, int i, float p) { x.f[i >> 3][i & 7] = (__bf16)p; }   // probabilities enter the matrix pipe as bf16
+    // Which channels a result block holds: rows 0 .. 15 of block d are the channels 16 d .., rows 16 .. 31 the channels DP / 2 + 16 d .. : the four
+    // 16-lane groups of a transposing read then touch different banks (rows are one chunk apart, the two column groups half a row): 2 instead of
+    // 8 cycles of LDS a read.
+    template <int DP> static __device__ __forceinline__ int channel(int d, int g4, int half) { return 16 * d + (g4 >> 1) * (DP / 2) + (g4 & 1) * 8 + 4 * half; }
     template <int DP> static __device__ __forceinline__ void value(f32x16 (&y)[DP / 32], const Cols& x, const char* w_l, int lane) {
         constexpr int ROW = DP * 2 + 16;
         const int half = lane >> 5, r16 = lane & 15, g16 = (lane >> 4) & 1;
-        const char* base = w_l + (4 * half + (r16 >> 2)) * ROW + (16 * g16 + 4 * (r16 & 3)) * 2;
+        const char* base = w_l + (4 * half + (r16 >> 2)) * ROW + (DP / 2 * g16 + 4 * (r16 & 3)) * 2;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) {
                 union { s16x4 h[2]; Frag f; } u;
-                const char* a = base + 16 * s * ROW + d * 64;
+                const char* a = base + 16 * s * ROW + d * 32;
                 u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
                 u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 8 * ROW));
                 y[d] = mma(u.f, x.f[s], y[d]);
             }
     }
-    template <int DP> static __device__ __forceinline__ f32x16 score(const char* rows_l, const Frag (&c)[DP / 16], int l31, int half) {
+    template <int DP> static __device__ __forceinline__ f32x16 score(const char* rows_l, const Frag (&c)[DP / 16], int l31, int half, f32x16 acc) {
         constexpr int ROW = DP * 2 + 16;
-        f32x16 acc;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) acc = mma(*reinterpret_cast<const Frag*>(rows_l + l31 * ROW + (16 * s + 8 * half) * 2), c[s], acc);
         return acc;
     }
     // the same with C's rows in LDS too
-    template <int DP> static __device__ __forceinline__ f32x16 score_lds(const char* rows_l, const char* c_l, int l31, int half) {
+    template <int DP> static __device__ __forceinline__ f32x16 score_lds(const char* rows_l, const char* c_l, int l31, int half, f32x16 acc) {
         constexpr int ROW = DP * 2 + 16;
-        f32x16 acc;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
             const int at = l31 * ROW + (16 * s + 8 * half) * 2;
@@ -100,6 +99,7 @@ template <> struct Op<float> {
     static __device__ __forceinline__ f32x16 mma(float a, float b, const f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
     struct Cols { f32x16 f; };
     static __device__ __forceinline__ void set(Cols& x, int i, float p) { x.f[i] = p; }
+    template <int DP> static __device__ __forceinline__ int channel(int d, int g4, int half) { return 32 * d + g4 * 8 + 4 * half; }
     template <int DP> static __device__ __forceinline__ void value(f32x16 (&y)[DP / 32], const Cols& x, const char* w_l, int lane) {
         constexpr int ROW = DP * 4 + 16;
         const int half = lane >> 5, l31 = lane & 31;
@@ -109,11 +109,8 @@ template <> struct Op<float> {
             for (int d = 0; d < DP / 32; ++d)
                 y[d] = mma(*reinterpret_cast<const float*>(w_l + ((i >> 2) * 8 + 4 * half + (i & 3)) * ROW + (d * 32 + l31) * 4), x.f[i], y[d]);
     }
-    template <int DP> static __device__ __forceinline__ f32x16 score(const char* rows_l, const Frag (&c)[DP / 8], int l31, int half) {
+    template <int DP> static __device__ __forceinline__ f32x16 score(const char* rows_l, const Frag (&c)[DP / 8], int l31, int half, f32x16 acc) {
         constexpr int ROW = DP * 4 + 16;
-        f32x16 acc;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
 #pragma unroll
         for (int g = 0; g < DP / 8; ++g) {
             const Frag r = *reinterpret_cast<const Frag*>(rows_l + l31 * ROW + (8 * g + 4 * half) * 4);
@@ -124,32 +121,47 @@ template <> struct Op<float> {
     }
 };
 
-// register fragments (B operand of a score product) of one row; channels from D on are zeros
+// Up to R rows of one head behind a buffer descriptor: what lies behind the last valid row or behind channel D reads as zeros, without a branch.
+// (Offsets inside a tile stay below 2^31: at most 128 rows of less than 2^24 bytes, checked on the host.)
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* base, int64_t row_stride, int rows) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    const int bytes = __builtin_amdgcn_readfirstlane(max(rows, 0) * (int)(row_stride * (int64_t)sizeof(T)));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0, bytes, 0x00020000);
+}
+constexpr int OUT = (int)0x80000000;         // an offset no descriptor reaches
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 buffer_chunk(__amdgpu_buffer_rsrc_t b, int offset) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0));
+}
+
+// register fragments (B operand of a score product) of row `row` of a buffer
 template <typename T, int DP>
-__device__ __forceinline__ void load_frags(typename Op<T>::Frag (&f)[Op<T>::template NF<DP>], const T* row, bool valid, int D, int half) {
+__device__ __forceinline__ void load_frags(typename Op<T>::Frag (&f)[Op<T>::template NF<DP>], __amdgpu_buffer_rsrc_t b, int64_t row_stride, int row, int D, int half) {
     typedef typename Op<T>::Frag Frag;
     constexpr int E = Op<T>::EPC;
+    const int at = row * (int)(row_stride * (int64_t)sizeof(T));
 #pragma unroll
     for (int s = 0; s < Op<T>::template NF<DP>; ++s) {
         const int d = (2 * s + half) * E;
-        Frag x = {};
-        if (valid && d < D) x = *reinterpret_cast<const Frag*>(row + d);
-        f[s] = x;
+        f[s] = __builtin_bit_cast(Frag, buffer_chunk(b, d < D ? at + d * (int)sizeof(T) : OUT));
     }
 }
 
 // R rows of one head -> LDS in two halves: request into registers, store later.  Row stride in LDS: DP elements and 16 bytes (a shift of four banks
-// from row to row).  Rows from nvalid on and channels from D on are zeros: what lies behind a document never enters a product.
+// from row to row).  Rows from `rows` on and channels from D on are zeros: what lies behind a document never enters a product.
 template <typename T, int DP, int R, int NT>
 struct Stage {
     static constexpr int E = Op<T>::EPC, CPR = DP / E, CHUNKS = R * CPR, N = (CHUNKS + NT - 1) / NT;
     f32x4 x[N];
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int row0, int nvalid, int D, int tid) {
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int rows, int D, int tid) {
+        const __amdgpu_buffer_rsrc_t b = row_buffer(base, row_stride, min(rows, R));
+        const int rb = (int)(row_stride * (int64_t)sizeof(T));
 #pragma unroll
         for (int it = 0; it < N; ++it) {
             const int i = tid + it * NT, r = i / CPR, c = i - r * CPR;
-            x[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if ((CHUNKS % NT == 0 || i < CHUNKS) && row0 + r < nvalid && c * E < D) x[it] = *reinterpret_cast<const f32x4*>(base + (int64_t)(row0 + r) * row_stride + c * E);
+            x[it] = buffer_chunk(b, c * E < D && (CHUNKS % NT == 0 || i < CHUNKS) ? r * rb + c * 16 : OUT);
         }
     }
     __device__ __forceinline__ void store(char* dst, int tid) const {
@@ -172,41 +184,48 @@ __device__ __forceinline__ void half_swap(float v, float& lo, float& hi) {
 __device__ __forceinline__ float half_max(float v) { float a, b; half_swap(v, a, b); return fmaxf(a, b); }
 __device__ __forceinline__ float half_sum(float v) { float a, b; half_swap(v, a, b); return a + b; }
 
-// The score function of one raw product x = q . k, in log2 units.
-//   EXACT (f32 tensors): tanh by the library;  otherwise 1 - 2 / (exp(2 y) + 1) on v_exp_f32 and v_rcp_f32, off by 2^-23 of the cap at most
-//   slope of the cap, d c / d x = 1 - tanh^2, returned where wanted
-struct Score {
-    float c1, c2, slope2;                 // plain: c1 = scale log2 e;  cap: c1 = 2 scale log2 e / cap (EXACT: scale / cap), c2 = cap log2 e
-    template <int MODE, bool EXACT> __device__ __forceinline__ float value(float x, float distance) const {
-        float s;
-        if constexpr (MODE & CAP) {
-            if constexpr (EXACT) s = c2 * tanhf(x * c1);
-            else s = fmaf(-2.f * c2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f), c2);
-        } else s = x * c1;
-        if constexpr (MODE & SLOPE) s = fmaf(-slope2, fabsf(distance), s);
-        return s;
-    }
-    template <int MODE, bool EXACT> __device__ __forceinline__ float value_and_slope(float x, float distance, float& g) const {
-        float s;
-        g = 1.f;
-        if constexpr (MODE & CAP) {
-            if constexpr (EXACT) { const float t = tanhf(x * c1); s = c2 * t; g = fmaf(-t, t, 1.f); }
-            else { const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f); s = fmaf(-2.f * c2, r, c2); g = 4.f * fmaf(-r, r, r); }
-        } else s = x * c1;
-        if constexpr (MODE & SLOPE) s = fmaf(-slope2, fabsf(distance), s);
-        return s;
-    }
-};
-template <int MODE, bool EXACT> __device__ __forceinline__ Score make_score(const Args& p, int head) {
-    Score s;
-    s.c1 = p.scale * LOG2E; s.c2 = 0.f; s.slope2 = 0.f;
-    if constexpr (MODE & CAP) {
-        s.c1 = EXACT ? p.scale / p.softcap : 2.f * p.scale * LOG2E / p.softcap;
-        s.c2 = p.softcap * LOG2E;
-    }
-    if constexpr (MODE & SLOPE) s.slope2 = p.slopes[head] * LOG2E;
-    return s;
+__device__ __forceinline__ f32x16 splat(float v) {
+    f32x16 x;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = v;
+    return x;
 }
+
+// The score function of a raw product x = q . k (scale > 0), in log2 units, as  s = a u + b:
+//   plain: u = x, a = scale log2 e;   cap: u = -1 / (exp(2 y) + 1) with y = scale x / cap, a = 2 cap log2 e, b = cap log2 e  (cap tanh y = cap - 2 cap / (exp
+//   2 y + 1) on v_exp_f32 and v_rcp_f32: off by 2^-22 of the cap at most);  EXACT (f32 tensors): u = tanh y by the library, a = cap log2 e
+//   slope: u becomes the score itself with the distance's penalty, a = 1, b = 0
+// A maximum over u is a maximum over s, and a u + b - max is one FMA in front of the exponential.
+// The cap's derivative 1 - tanh^2 y is 4 (-u - u u) for the first form: the factor 4 goes to the caller (grad_scale).
+template <int MODE, bool EXACT>
+struct Score {
+    float c1, a, b, fa, fb, slope2;
+    __device__ __forceinline__ Score(const Args& p, int head) {
+        c1 = 0.f; slope2 = 0.f;
+        if constexpr (!(MODE & CAP)) { a = p.scale * LOG2E; b = 0.f; }
+        else if constexpr (EXACT) { c1 = p.scale / p.softcap; a = p.softcap * LOG2E; b = 0.f; }
+        else { c1 = 2.f * p.scale * LOG2E / p.softcap; a = 2.f * p.softcap * LOG2E; b = p.softcap * LOG2E; }
+        fa = a; fb = b;
+        if constexpr (MODE & SLOPE) { fa = 1.f; fb = 0.f; }
+        set_head(p, head);
+    }
+    __device__ __forceinline__ void set_head(const Args& p, int head) { if constexpr (MODE & SLOPE) slope2 = p.slopes[head] * LOG2E; }
+    __device__ __forceinline__ float cap(float x) const {
+        if constexpr (!(MODE & CAP)) return x;
+        if constexpr (EXACT) return tanhf(x * c1);
+        return -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f);
+    }
+    __device__ __forceinline__ float penalise(float u, float distance) const {
+        if constexpr (MODE & SLOPE) return fmaf(u, a, fmaf(-slope2, fabsf(distance), b));
+        return u;
+    }
+    // derivative of the capped score by the raw one, from cap(x), without grad_scale
+    __device__ __forceinline__ float derive(float c) const { return EXACT ? fmaf(-c, c, 1.f) : fmaf(-c, c, -c); }
+    static constexpr float grad_scale = (MODE & CAP) && !EXACT ? 4.f : 1.f;
+};
+
+// host: a tile's rows fit a buffer descriptor, and a row reaches no further than the next
+static inline bool row_stride_ok(int64_t stride, int64_t D, int64_t bf16) { return stride >= D && stride * (bf16 ? 2 : 4) < (int64_t)1 << 24; }
 
 // keys a query at position pos sees
 __device__ __forceinline__ int key_limit(int pos, int klen, int prefix, int causal) {

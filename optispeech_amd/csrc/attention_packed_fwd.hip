@@ -1,5 +1,7 @@
 // Attention over documents, forward: capped scores, a penalty on distance, document, causal and prefix masks, shared key heads.
-// Scores and masks: attention_packed_common.h.  Besides o the kernel keeps one number per query and head, the log2-sum-exp of its scores.
+// Scores and masks: attention_packed_common.h.  For a backward the kernel keeps one number per query and head, the log2-sum-exp of its scores, and for
+// bf16 results what their rounding took off (`rest`, bf16): the backward's delta = sum dO O would otherwise carry that rounding into every
+// element of a row of dS alike.
 //
 // One workgroup = 4 waves = one tile of 128 queries of one head; a wave owns 32 queries (one per lane, both halves of the wave hold the same
 // query and half of the keys).  Keys and values pass through LDS in tiles (64 rows, f32: 32), two buffers, one barrier per tile: the next tile's
@@ -8,6 +10,7 @@
 // The running maximum is moved only when a row's maximum grows by more than 8 (a factor of 256 in the probabilities, which f32 sums and bf16
 // operands carry without loss): the rescaling of O is skipped for nearly every tile after the first.
 #include "attention_packed_common.h"
+#include <type_traits>
 
 namespace {
 using namespace pattn;
@@ -43,8 +46,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
     const int wmax = w0 < tile.n ? max(key_limit(off + min(w0 + 31, tile.n - 1), klen, prefix, p.causal), 0) : 0;   // ... of the wave
     const int wmin = key_limit(off + w0, klen, prefix, p.causal);                      // keys every query of the wave sees
     typename O::Frag qf[O::template NF<DP>];
-    load_frags<T, DP>(qf, reinterpret_cast<const T*>(p.q) + qrow * p.qr + (int64_t)h * p.qh, qi < tile.n, p.D, half);
-    const Score sc = make_score<MODE, EXACT>(p, h);
+    load_frags<T, DP>(qf, row_buffer(reinterpret_cast<const T*>(p.q) + (int64_t)tile.row0 * p.qr + (int64_t)h * p.qh, p.qr, tile.n), p.qr, qi, p.D, half);
+    const Score<MODE, EXACT> sc(p, h);
     f32x16 oacc[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -54,11 +57,11 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
     const int nt = (kmax + KT - 1) / KT;
     Stage<T, DP, KT, 256> ks, vs;
     if (nt > 0) {
-        ks.load(kp, p.kr, 0, klen, p.D, tid);
-        vs.load(vp, p.vr, 0, klen, p.D, tid);
+        ks.load(kp, p.kr, klen, p.D, tid);
+        vs.load(vp, p.vr, klen, p.D, tid);
         ks.store(lds[0][0], tid);
         vs.store(lds[0][1], tid);
-        if (nt > 1) { ks.load(kp, p.kr, KT, klen, p.D, tid); vs.load(vp, p.vr, KT, klen, p.D, tid); }
+        if (nt > 1) { ks.load(kp + KT * p.kr, p.kr, klen - KT, p.D, tid); vs.load(vp + KT * p.vr, p.vr, klen - KT, p.D, tid); }
     }
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
@@ -67,24 +70,25 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
         if (k0 < wmax) {
             f32x16 st[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) st[b] = O::template score<DP>(kl + b * 32 * ROW, qf, l31, half);
-            const float dist = (float)(pos - k0 - 4 * half);
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) st[b][i] = sc.template value<MODE, EXACT>(st[b][i], dist - (float)(b * 32 + (i >> 2) * 8 + (i & 3)));
-            if (k0 + KT > wmin) {                                                      // some query of the wave does not see the whole tile
+            for (int b = 0; b < NB; ++b) st[b] = O::template score<DP>(kl + b * 32 * ROW, qf, l31, half, splat(0.f));
+            float mx = -INFINITY;
+            const int left = lim - k0 - 4 * half;                                      // rows of the tile this lane's query sees
+            auto elements = [&](auto masked) {
+                float at = (float)(pos - k0 - 4 * half);
+                if constexpr (MODE & SLOPE) asm volatile("" : "+v"(at));              // keeps a whole tile's penalties from being computed ahead of the branch
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) st[b][i] = k0 + b * 32 + (i >> 2) * 8 + 4 * half + (i & 3) < lim ? st[b][i] : -INFINITY;
-            }
-            float mx = st[0][0];
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[b][i]);
-            mx = half_max(mx);
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = b * 32 + (i >> 2) * 8 + (i & 3);
+                        float s = sc.penalise(sc.cap(st[b][i]), at - (float)r);
+                        if constexpr (masked) s = r < left ? s : -INFINITY;
+                        st[b][i] = s;
+                        mx = fmaxf(mx, s);
+                    }
+            };
+            if (k0 + KT > wmin) elements(std::true_type{}); else elements(std::false_type{});   // (where every query sees the whole tile)
+            mx = fmaf(half_max(mx), sc.fa, sc.fb);
             if (__any(mx > m_run + 8.f)) {
                 const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
                 m_run = m_new;
@@ -94,12 +98,13 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) oacc[d][i] *= alpha;
             }
+            const float shift = sc.fb - m_run;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 typename O::Cols pc;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(st[b][i] - m_run);
+                    const float e = __builtin_amdgcn_exp2f(fmaf(st[b][i], sc.fa, shift));
                     l_run += e;
                     O::set(pc, i, e);
                 }
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
         if (t + 1 < nt) {
             ks.store(lds[(t + 1) & 1][0], tid);
             vs.store(lds[(t + 1) & 1][1], tid);
-            if (t + 2 < nt) { ks.load(kp, p.kr, k0 + 2 * KT, klen, p.D, tid); vs.load(vp, p.vr, k0 + 2 * KT, klen, p.D, tid); }
+            if (t + 2 < nt) { ks.load(kp + (int64_t)(k0 + 2 * KT) * p.kr, p.kr, klen - k0 - 2 * KT, p.D, tid); vs.load(vp + (int64_t)(k0 + 2 * KT) * p.vr, p.vr, klen - k0 - 2 * KT, p.D, tid); }
         }
         __syncthreads();
     }
@@ -120,9 +125,17 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int c = d * 32 + g * 8 + 4 * half;
+            const int c = O::template channel<DP>(d, g, half);
             const float r[4] = {oacc[d][4 * g] * inv, oacc[d][4 * g + 1] * inv, oacc[d][4 * g + 2] * inv, oacc[d][4 * g + 3] * inv};
-            if (c < p.D) PackedVec<T, 4>::store(out + c, r);
+            if (c < p.D) {
+                PackedVec<T, 4>::store(out + c, r);
+                if constexpr (!EXACT) {
+                    if (p.rest) {
+                        const float e[4] = {r[0] - (float)(T)r[0], r[1] - (float)(T)r[1], r[2] - (float)(T)r[2], r[3] - (float)(T)r[3]};
+                        PackedVec<T, 4>::store(reinterpret_cast<T*>(p.rest) + (qrow * p.Hq + h) * p.D + c, e);
+                    }
+                }
+            }
         }
 }
 
@@ -146,7 +159,7 @@ void launch_width(const Args& p, hipStream_t s) {
 }  // namespace
 
 extern "C" int osp_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
-                                        int64_t v_row, int64_t v_head, int64_t bf16, void* o, float* lse, const int64_t* qlen, const int32_t* qtiles,
+                                        int64_t v_row, int64_t v_head, int64_t bf16, void* o, void* rest, float* lse, const int64_t* qlen, const int32_t* qtiles,
                                         const int32_t* qntiles, int64_t qcap, const int64_t* kbegin, const int64_t* klen, const int64_t* prefix,
                                         const float* slopes, int64_t Mq, int64_t Hq, int64_t Hk, int64_t D, float scale, float softcap, int64_t causal,
                                         hipStream_t stream) {
@@ -156,9 +169,10 @@ extern "C" int osp_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_
     const int E = bf16 ? 8 : 4;
     OSP_CHECK_ARG(q_row % E == 0 && q_head % E == 0 && k_row % E == 0 && k_head % E == 0 && v_row % E == 0 && v_head % E == 0 && packed_aligned(q, 16) &&
                   packed_aligned(k, 16) && packed_aligned(v, 16) && packed_aligned(o, 16), "rows and heads must start on 16 bytes");
-    OSP_CHECK_ARG(qcap > 0 && qcap * Hq < (int64_t)1 << 31 && softcap >= 0.f && (causal || !prefix), "bad tile list, cap or mask");
+    OSP_CHECK_ARG(qcap > 0 && qcap * Hq < (int64_t)1 << 31 && scale > 0.f && softcap >= 0.f && (causal || !prefix), "bad tile list, cap or mask");
+    OSP_CHECK_ARG(row_stride_ok(q_row, D, bf16) && row_stride_ok(k_row, D, bf16) && row_stride_ok(v_row, D, bf16), "row strides must lie between the head width and 2^24 bytes");
     Args p = {};
-    p.q = q; p.k = k; p.v = v; p.out = o; p.lse = lse;
+    p.q = q; p.k = k; p.v = v; p.out = o; p.rest = rest; p.lse = lse;
     p.qr = q_row; p.qh = q_head; p.kr = k_row; p.kh = k_head; p.vr = v_row; p.vh = v_head;
     p.qlen = qlen; p.kbegin = kbegin; p.klen = klen; p.tiles = reinterpret_cast<const PackedTile*>(qtiles); p.ntiles = qntiles;
     p.prefix = prefix; p.slopes = slopes; p.Mq = Mq; p.cap_tiles = (int)qcap; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk); p.D = (int)D;

@@ -36,8 +36,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_token
         const int h = hk * p.G + (on ? g : 0);
         const int64_t qrow = qb + (on ? i : 0);
         typename O::Frag qf[O::template NF<DP>];
-        load_frags<T, DP>(qf, reinterpret_cast<const T*>(p.q) + qrow * p.qr + (int64_t)h * p.qh, on, p.D, half);
-        const Score sc = make_score<MODE, EXACT>(p, h);
+        const T* qp = reinterpret_cast<const T*>(p.q) + qrow * p.qr + (int64_t)h * p.qh;     // rows of several heads and queries: no common buffer
+#pragma unroll
+        for (int s = 0; s < O::template NF<DP>; ++s) {
+            const int d = (2 * s + half) * O::EPC;
+            typename O::Frag x = {};
+            if (on && d < p.D) x = *reinterpret_cast<const typename O::Frag*>(qp + d);
+            qf[s] = x;
+        }
+        const Score<MODE, EXACT> sc(p, h);
         const int pos = klen - qlen + i, lim = on ? key_limit(pos, klen, prefix, p.causal) : 0;
         f32x16 oacc[DP / 32];
 #pragma unroll
@@ -47,25 +54,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_token
         float m_run = NONE, l_run = 0.f;
         Stage<T, DP, 32, 64> ks, vs;
         int k0 = k_lo + wave * 32;
-        if (k0 < k_hi) { ks.load(kp, p.kr, k0, k_hi, p.D, lane); vs.load(vp, p.vr, k0, k_hi, p.D, lane); }
+        if (k0 < k_hi) { ks.load(kp + (int64_t)k0 * p.kr, p.kr, k_hi - k0, p.D, lane); vs.load(vp + (int64_t)k0 * p.vr, p.vr, k_hi - k0, p.D, lane); }
         for (; k0 < k_hi; k0 += 128) {
             __builtin_amdgcn_wave_barrier();
             ks.store(kl, lane);
             vs.store(vl, lane);
             __builtin_amdgcn_wave_barrier();
-            if (k0 + 128 < k_hi) { ks.load(kp, p.kr, k0 + 128, k_hi, p.D, lane); vs.load(vp, p.vr, k0 + 128, k_hi, p.D, lane); }
-            f32x16 st = O::template score<DP>(kl, qf, l31, half);
+            if (k0 + 128 < k_hi) { ks.load(kp + (int64_t)(k0 + 128) * p.kr, p.kr, k_hi - k0 - 128, p.D, lane); vs.load(vp + (int64_t)(k0 + 128) * p.vr, p.vr, k_hi - k0 - 128, p.D, lane); }
+            f32x16 st = O::template score<DP>(kl, qf, l31, half, splat(0.f));
             const float dist = (float)(pos - k0 - 4 * half);
             const int left = min(lim, k_hi) - k0 - 4 * half;
             float mx = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int r = (e >> 2) * 8 + (e & 3);
-                const float s = sc.template value<MODE, EXACT>(st[e], dist - (float)r);
+                const float s = sc.penalise(sc.cap(st[e]), dist - (float)r);
                 st[e] = r < left ? s : -INFINITY;
                 mx = fmaxf(mx, st[e]);
             }
-            mx = half_max(mx);
+            mx = fmaf(half_max(mx), sc.fa, sc.fb);
             if (__any(mx > m_run + 8.f)) {
                 const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
                 m_run = m_new;
@@ -76,9 +83,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_token
                     for (int e = 0; e < 16; ++e) oacc[d][e] *= alpha;
             }
             typename O::Cols pc;
+            const float shift = sc.fb - m_run;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float x = __builtin_amdgcn_exp2f(st[e] - m_run);
+                const float x = __builtin_amdgcn_exp2f(fmaf(st[e], sc.fa, shift));
                 l_run += x;
                 O::set(pc, e, x);
             }
@@ -96,7 +104,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_token
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
-                *reinterpret_cast<f32x4*>(mine + l31 * DP + d * 32 + q4 * 8 + 4 * half) =
+                *reinterpret_cast<f32x4*>(mine + l31 * DP + O::template channel<DP>(d, q4, half)) =
                     f32x4{oacc[d][4 * q4] * f, oacc[d][4 * q4 + 1] * f, oacc[d][4 * q4 + 2] * f, oacc[d][4 * q4 + 3] * f};
         __syncthreads();
         const int nc = min(32, cols - c0);
@@ -196,7 +204,8 @@ extern "C" int osp_packed_attention_token(const void* q, int64_t q_row, int64_t 
     const int E = bf16 ? 8 : 4;
     OSP_CHECK_ARG(q_row % E == 0 && q_head % E == 0 && k_row % E == 0 && k_head % E == 0 && v_row % E == 0 && v_head % E == 0 && packed_aligned(q, 16) &&
                   packed_aligned(k, 16) && packed_aligned(v, 16) && packed_aligned(o, 16) && packed_aligned(workspace, 16), "rows and heads must start on 16 bytes");
-    OSP_CHECK_ARG(qcap > 0 && qcap < (int64_t)1 << 31 && softcap >= 0.f && (causal || !prefix), "bad tile list, cap or mask");
+    OSP_CHECK_ARG(qcap > 0 && qcap < (int64_t)1 << 31 && scale > 0.f && softcap >= 0.f && (causal || !prefix), "bad tile list, cap or mask");
+    OSP_CHECK_ARG(row_stride_ok(q_row, D, bf16) && row_stride_ok(k_row, D, bf16) && row_stride_ok(v_row, D, bf16), "row strides must lie between the head width and 2^24 bytes");
     Args p = {};
     p.q = q; p.k = k; p.v = v; p.out = o;
     p.qr = q_row; p.qh = q_head; p.kr = k_row; p.kh = k_head; p.vr = v_row; p.vh = v_head;

@@ -270,18 +270,20 @@ def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
 
 # ------------------------------------------------------------------------------------------------------------------ attention over documents
 def _aligned(t, name):
-    """(M, heads, width) whose rows and heads start on 16 bytes (the kernels' access): a copy where they do not."""
+    """(M, heads, width) whose rows and heads start on 16 bytes and whose rows do not overlap (the kernels' access): a copy where they do not."""
     t = _heads(t, name)
     e = 16 // t.element_size()
-    return t if t.stride(0) % e == 0 and t.stride(1) % e == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
+    r, h = t.stride(0), t.stride(1)
+    return t if r % e == 0 and h % e == 0 and t.data_ptr() % 16 == 0 and t.shape[2] <= r < 1 << 22 else t.contiguous()
 
 
 def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):
-    """-> (q, k, v as the kernels read them, o, log2-sum-exp or None)"""
+    """-> (q, k, v as the kernels read them, o, what o's rounding took off (bf16) and the log2-sum-exp where a backward wants them)"""
     q, k, v = _aligned(q, "q"), _aligned(k, "k"), _aligned(v, "v")
     (M, H, D), S, bf16 = q.shape, k.shape[1], int(q.dtype == torch.bfloat16)
     o = torch.empty((M, H, D), device=q.device, dtype=q.dtype)
     lse = torch.empty((H, M), device=q.device, dtype=torch.float32) if save else None
+    rest = torch.empty_like(o) if save and bf16 else None
     if M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536:
         # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip)
         ws = _workspace(_size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D), q.device)
@@ -289,22 +291,22 @@ def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):
              rows.begin, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, keys.longest, prefix, slopes, rows.docs, M, H, S,
              D, scale, softcap, causal)
     elif M:
-        call("osp_packed_attention_fwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, lse,
-             rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, prefix, slopes, M, H, S, D, scale, softcap, causal)
-    return q, k, v, o, lse
+        call("osp_packed_attention_fwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, rest,
+             lse, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, prefix, slopes, M, H, S, D, scale, softcap, causal)
+    return q, k, v, o, rest, lse
 
 
 class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, rows, keys, causal, prefix, softcap, slopes, scale):
-        q, k, v, o, lse = _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse, prefix, slopes)
+        q, k, v, o, rest, lse = _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, True)
+        ctx.save_for_backward(q, k, v, o, rest, lse, prefix, slopes)
         ctx.cfg = (rows, keys, causal, softcap, scale)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse, prefix, slopes = ctx.saved_tensors
+        q, k, v, o, rest, lse, prefix, slopes = ctx.saved_tensors
         rows, keys, causal, softcap, scale = ctx.cfg
         (M, H, D), (Mk, S, _) = q.shape, k.shape
         do = _aligned(do, "the gradient of o")
@@ -312,7 +314,7 @@ class PackedAttentionFn(torch.autograd.Function):
         dk, dv = (torch.empty((Mk, S, D), device=q.device, dtype=q.dtype) for _ in range(2))
         if M and Mk:
             delta = torch.empty_like(lse)
-            call("osp_packed_attention_bwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), o, lse, do,
+            call("osp_packed_attention_bwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), o, rest, lse, do,
                  do.stride(0), do.stride(1), int(q.dtype == torch.bfloat16), dq, dk, dv, delta, rows.begin, rows.length, rows.tiles, rows.ntiles,
                  rows.cap, keys.begin, keys.length, keys.tiles, keys.ntiles, keys.cap, prefix, slopes, M, H, S, D, scale, softcap, causal)
         else:
@@ -327,7 +329,7 @@ def attention(q, k, v, rows, keys=None, causal=False, prefix=None, softcap=0.0, 
     ``rows`` (PackedRows) lays out the queries; ``keys`` the keys where they differ (a cache: ``PackedRows.from_padded(lengths, capacity)``), with the
     same number of documents.  Query i of a document stands at position  keys - queries + i : the last query is at the last key.
 
-    score = c(scale q . k) - slopes[head] |position - j|, with c(x) = softcap tanh(x / softcap) where softcap > 0; scale 1 / sqrt(width) unless given;
+    score = c(scale q . k) - slopes[head] |position - j|, with c(x) = softcap tanh(x / softcap) where softcap > 0; scale (positive) 1 / sqrt(width) unless given;
     slopes (heads,) float32 (no gradient).  ``causal``: key j is seen from position j on; ``prefix`` (docs,) int64 with it: the first prefix keys of
     a document are seen by all its queries.  A query that sees nothing gives zeros, and so do rows of no document; gradients likewise.
     Keys and values must be finite where any query sees them; what lies behind a document is never read into a product.
@@ -350,8 +352,8 @@ def attention(q, k, v, rows, keys=None, causal=False, prefix=None, softcap=0.0, 
     if not softcap >= 0.0 or math.isinf(softcap):
         raise OspError(f"softcap {softcap}: positive, or 0 for none")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise OspError(f"scale {scale}")
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise OspError(f"scale {scale}: positive")
     keys = rows if keys is None else keys
     rows._check(q, "q")
     keys._check(k, "k")
