@@ -72,14 +72,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_ke
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    settle(qf);
+    settle(dof);
     const int nt = (kmax + KT - 1) / KT;
-    Stage<T, DP, KT, 256> ks, vs;
+    Stage<T, DP, KT, 256> ks(p.kr, p.D, tid), vs(p.vr, p.D, tid);
     if (nt > 0) {
-        ks.load(kp, p.kr, klen, p.D, tid);
-        vs.load(vp, p.vr, klen, p.D, tid);
+        ks.load(kp, p.kr, klen);
+        vs.load(vp, p.vr, klen);
         ks.store(lds[0][0], tid);
         vs.store(lds[0][1], tid);
-        if (nt > 1) { ks.load(kp + KT * p.kr, p.kr, klen - KT, p.D, tid); vs.load(vp + KT * p.vr, p.vr, klen - KT, p.D, tid); }
+        if (nt > 1) { ks.load(kp + KT * p.kr, p.kr, klen - KT); vs.load(vp + KT * p.vr, p.vr, klen - KT); }
     }
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_ke
         if (t + 1 < nt) {
             ks.store(lds[(t + 1) & 1][0], tid);
             vs.store(lds[(t + 1) & 1][1], tid);
-            if (t + 2 < nt) { ks.load(kp + (int64_t)(k0 + 2 * KT) * p.kr, p.kr, klen - k0 - 2 * KT, p.D, tid); vs.load(vp + (int64_t)(k0 + 2 * KT) * p.vr, p.vr, klen - k0 - 2 * KT, p.D, tid); }
+            if (t + 2 < nt) { ks.load(kp + (int64_t)(k0 + 2 * KT) * p.kr, p.kr, klen - k0 - 2 * KT); vs.load(vp + (int64_t)(k0 + 2 * KT) * p.vr, p.vr, klen - k0 - 2 * KT); }
         }
         __syncthreads();
     }
@@ -170,10 +172,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_k
     load_frags<T, DP>(kf, row_buffer(reinterpret_cast<const T*>(p.k) + (int64_t)tile.row0 * p.kr + (int64_t)hk * p.kh, p.kr, tile.n), p.kr, ki, p.D, half);
     const T* vrows = reinterpret_cast<const T*>(p.v) + (int64_t)tile.row0 * p.vr + (int64_t)hk * p.vh;
     if constexpr (VLDS) {
-        Stage<T, DP, PACKED_TILE, 256> vs;
-        vs.load(vrows, p.vr, tile.n, p.D, tid);
+        Stage<T, DP, PACKED_TILE, 256> vs(p.vr, p.D, tid);
+        vs.load(vrows, p.vr, tile.n);
         vs.store(v_l, tid);
     } else load_frags<T, DP>(vf, row_buffer(vrows, p.vr, tile.n), p.vr, ki, p.D, half);
+    settle(kf);
+    if constexpr (!VLDS) settle(vf);
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -183,12 +187,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_k
     const int nqt = first < qlen ? (qlen - first + QT - 1) / QT : 0, nt = nqt * p.G;
     Score<MODE, EXACT> sc(p, hk * p.G);
     const float back = p.scale * sc.grad_scale;
-    Stage<T, DP, QT, 256> qs, dos;
+    Stage<T, DP, QT, 256> qs(p.qr, p.D, tid), dos(p.dor, p.D, tid);
     float st_reg = 0.f;
     auto load = [&](int t) {
         const int h = hk * p.G + t / nqt, r0 = first + (t % nqt) * QT;
-        qs.load(reinterpret_cast<const T*>(p.q) + (qb + r0) * p.qr + (int64_t)h * p.qh, p.qr, qlen - r0, p.D, tid);
-        dos.load(reinterpret_cast<const T*>(p.dout) + (qb + r0) * p.dor + (int64_t)h * p.doh, p.dor, qlen - r0, p.D, tid);
+        qs.load(reinterpret_cast<const T*>(p.q) + (qb + r0) * p.qr + (int64_t)h * p.qh, p.qr, qlen - r0);
+        dos.load(reinterpret_cast<const T*>(p.dout) + (qb + r0) * p.dor + (int64_t)h * p.doh, p.dor, qlen - r0);
         if (tid < 2 * QT) {
             const int r = r0 + (tid & (QT - 1));
             const float* src = tid < QT ? p.lse : p.delta;

@@ -149,20 +149,35 @@ __device__ __forceinline__ void load_frags(typename Op<T>::Frag (&f)[Op<T>::temp
     }
 }
 
+// Fragments that a loop reads are waited for in front of it: a wait left to their first use would stand in the loop and, from the second turn on, wait
+// for the loads that were sent ahead for the next tile.
+template <typename F, int N>
+__device__ __forceinline__ void settle(F (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 // R rows of one head -> LDS in two halves: request into registers, store later.  Row stride in LDS: DP elements and 16 bytes (a shift of four banks
 // from row to row).  Rows from `rows` on and channels from D on are zeros: what lies behind a document never enters a product.
 template <typename T, int DP, int R, int NT>
 struct Stage {
     static constexpr int E = Op<T>::EPC, CPR = DP / E, CHUNKS = R * CPR, N = (CHUNKS + NT - 1) / NT;
+    static constexpr bool EVEN = NT % CPR == 0;                          // a thread's chunks lie NT / CPR rows apart: one offset and a step
     f32x4 x[N];
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int rows, int D, int tid) {
-        const __amdgpu_buffer_rsrc_t b = row_buffer(base, row_stride, min(rows, R));
+    int off[EVEN ? 1 : N], step;
+    __device__ __forceinline__ Stage(int64_t row_stride, int D, int tid) {
         const int rb = (int)(row_stride * (int64_t)sizeof(T));
+        step = NT / CPR * rb;
 #pragma unroll
-        for (int it = 0; it < N; ++it) {
+        for (int it = 0; it < (EVEN ? 1 : N); ++it) {
             const int i = tid + it * NT, r = i / CPR, c = i - r * CPR;
-            x[it] = buffer_chunk(b, c * E < D && (CHUNKS % NT == 0 || i < CHUNKS) ? r * rb + c * 16 : OUT);
+            off[it] = c * E < D && i < CHUNKS ? r * rb + c * 16 : OUT;   // (OUT and a few steps stay out of reach)
         }
+    }
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int rows) {
+        const __amdgpu_buffer_rsrc_t b = row_buffer(base, row_stride, min(rows, R));
+#pragma unroll
+        for (int it = 0; it < N; ++it) x[it] = buffer_chunk(b, EVEN ? off[0] + it * step : off[EVEN ? 0 : it]);
     }
     __device__ __forceinline__ void store(char* dst, int tid) const {
         constexpr int ROW = DP * (int)sizeof(T) + 16;

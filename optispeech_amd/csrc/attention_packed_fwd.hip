@@ -53,15 +53,16 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) oacc[d][i] = 0.f;
+    settle(qf);
     float m_run = NONE, l_run = 0.f;
     const int nt = (kmax + KT - 1) / KT;
-    Stage<T, DP, KT, 256> ks, vs;
+    Stage<T, DP, KT, 256> ks(p.kr, p.D, tid), vs(p.vr, p.D, tid);
     if (nt > 0) {
-        ks.load(kp, p.kr, klen, p.D, tid);
-        vs.load(vp, p.vr, klen, p.D, tid);
+        ks.load(kp, p.kr, klen);
+        vs.load(vp, p.vr, klen);
         ks.store(lds[0][0], tid);
         vs.store(lds[0][1], tid);
-        if (nt > 1) { ks.load(kp + KT * p.kr, p.kr, klen - KT, p.D, tid); vs.load(vp + KT * p.vr, p.vr, klen - KT, p.D, tid); }
+        if (nt > 1) { ks.load(kp + KT * p.kr, p.kr, klen - KT); vs.load(vp + KT * p.vr, p.vr, klen - KT); }
     }
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
         if (t + 1 < nt) {
             ks.store(lds[(t + 1) & 1][0], tid);
             vs.store(lds[(t + 1) & 1][1], tid);
-            if (t + 2 < nt) { ks.load(kp + (int64_t)(k0 + 2 * KT) * p.kr, p.kr, klen - k0 - 2 * KT, p.D, tid); vs.load(vp + (int64_t)(k0 + 2 * KT) * p.vr, p.vr, klen - k0 - 2 * KT, p.D, tid); }
+            if (t + 2 < nt) { ks.load(kp + (int64_t)(k0 + 2 * KT) * p.kr, p.kr, klen - k0 - 2 * KT); vs.load(vp + (int64_t)(k0 + 2 * KT) * p.vr, p.vr, klen - k0 - 2 * KT); }
         }
         __syncthreads();
     }

@@ -51,16 +51,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_token
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
+        settle(qf);
         float m_run = NONE, l_run = 0.f;
-        Stage<T, DP, 32, 64> ks, vs;
+        Stage<T, DP, 32, 64> ks(p.kr, p.D, lane), vs(p.vr, p.D, lane);
         int k0 = k_lo + wave * 32;
-        if (k0 < k_hi) { ks.load(kp + (int64_t)k0 * p.kr, p.kr, k_hi - k0, p.D, lane); vs.load(vp + (int64_t)k0 * p.vr, p.vr, k_hi - k0, p.D, lane); }
+        if (k0 < k_hi) { ks.load(kp + (int64_t)k0 * p.kr, p.kr, k_hi - k0); vs.load(vp + (int64_t)k0 * p.vr, p.vr, k_hi - k0); }
         for (; k0 < k_hi; k0 += 128) {
             __builtin_amdgcn_wave_barrier();
             ks.store(kl, lane);
             vs.store(vl, lane);
             __builtin_amdgcn_wave_barrier();
-            if (k0 + 128 < k_hi) { ks.load(kp + (int64_t)(k0 + 128) * p.kr, p.kr, k_hi - k0 - 128, p.D, lane); vs.load(vp + (int64_t)(k0 + 128) * p.vr, p.vr, k_hi - k0 - 128, p.D, lane); }
+            if (k0 + 128 < k_hi) { ks.load(kp + (int64_t)(k0 + 128) * p.kr, p.kr, k_hi - k0 - 128); vs.load(vp + (int64_t)(k0 + 128) * p.vr, p.vr, k_hi - k0 - 128); }
             f32x16 st = O::template score<DP>(kl, qf, l31, half, splat(0.f));
             const float dist = (float)(pos - k0 - 4 * half);
             const int left = min(lim, k_hi) - k0 - 4 * half;
