@@ -9,8 +9,8 @@
 // do 64-bit FMAs at the 32-bit rate and the kernel is bound by HBM).  The backward's per-channel sums run in 32 bits over the rows of one
 // workgroup (at most PACKED_TILE) and in 64 bits from there on.  Every sum has one fixed order: no atomics.
 //
-// Bound: HBM.  A document is larger than a CU can hold (800 rows x 256 channels x 4 bytes), so x is read twice, the second time mostly out of
-// the 256 MB last-level cache.  Forward: partial sums per (tile part, group) -> apply, whose workgroups add the few partials of their document
+// Bound: HBM.  Where a document's rows x one slab of groups fit the registers of a workgroup, one launch reads x (and dy) once: see "documents that fit".
+// Longer documents and groups that are no whole vectors are read twice, the second time mostly out of the 256 MB last-level cache.  Forward: partial sums per (tile part, group) -> apply, whose workgroups add the few partials of their document
 // themselves (a launch of its own does it where a document has many).  Backward: per-channel partials -> per-document sums -> apply, the
 // sum of the documents' dw / db riding on the last launch.
 #include "packed_common.h"
@@ -79,6 +79,15 @@ __device__ __forceinline__ Lanes lanes_of(int nvec) {
     l.ry = threadIdx.x / l.nx;
     l.cx = threadIdx.x - l.ry * l.nx;
     return l;
+}
+
+// n elements from y on become zeros, 16 bytes at a time where they start on 16 bytes
+template <typename T>
+__device__ __forceinline__ void zero_rows(T* y, int64_t n) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int64_t m = reinterpret_cast<uintptr_t>(y) % 16 == 0 ? n / E : 0;
+    for (int64_t i = threadIdx.x; i < m; i += blockDim.x) reinterpret_cast<float4*>(y)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t i = m * E + threadIdx.x; i < n; i += blockDim.x) y[i] = (T)0.f;
 }
 
 // sum over the lanes of aligned groups of L (a power of two)
@@ -177,10 +186,6 @@ __global__ __launch_bounds__(NTH) void gn_finish_kernel(const NormArgs p) {
     for (int g = threadIdx.x; g < p.G; g += NTH) { p.mean[(int64_t)doc * p.G + g] = mean_l[g]; p.rstd[(int64_t)doc * p.G + g] = rstd_l[g]; }
 }
 
-template <typename T>
-__device__ __forceinline__ void zero_rows(T* y, int64_t n) {
-    for (int64_t i = threadIdx.x; i < n; i += NTH) y[i] = (T)0.f;
-}
 
 // ------------------------------------------------------------------------------------------------ forward: apply
 template <typename T, int V, int ACT, bool DIRECT>
@@ -314,25 +319,28 @@ __global__ __launch_bounds__(512) void gn_bwd_docs_kernel(const NormArgs p, int 
     }
 }
 
+__device__ __forceinline__ void weight_sums(const NormArgs& p, int c0) {
+    __shared__ double2 red[4][64];
+    const int lane = threadIdx.x & 63, sl = threadIdx.x >> 6, c = c0 + lane;
+    double a = 0.0, b = 0.0;
+    if (c < p.C) {
+#pragma unroll 4
+        for (int d = sl; d < p.B; d += 4) { const double2 v = reinterpret_cast<const double2*>(p.dsum)[(int64_t)d * p.C + c]; a += v.x; b += v.y; }
+    }
+    red[sl][lane] = make_double2(a, b);
+    __syncthreads();
+    if (sl == 0 && c < p.C) {
+        for (int i = 1; i < 4; ++i) { a += red[i][lane].x; b += red[i][lane].y; }
+        if (p.db) p.db[c] = (float)a + (p.add_b ? p.db[c] : 0.f);
+        if (p.dw) p.dw[c] = (float)b + (p.add_w ? p.dw[c] : 0.f);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ backward: dx, and dw / db behind the tiles
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(NTH) void gn_bwd_apply_kernel(const NormArgs p) {
-    __shared__ double2 red[4][64];
-    if ((int)blockIdx.x >= p.cap) {              // the last workgroups: 64 channels each, the documents' sums in their order
-        if (blockIdx.y) return;
-        const int lane = threadIdx.x & 63, sl = threadIdx.x >> 6, c = ((int)blockIdx.x - p.cap) * 64 + lane;
-        double a = 0.0, b = 0.0;
-        if (c < p.C) {
-#pragma unroll 4
-            for (int d = sl; d < p.B; d += 4) { const double2 v = reinterpret_cast<const double2*>(p.dsum)[(int64_t)d * p.C + c]; a += v.x; b += v.y; }
-        }
-        red[sl][lane] = make_double2(a, b);
-        __syncthreads();
-        if (sl == 0 && c < p.C) {
-            for (int i = 1; i < 4; ++i) { a += red[i][lane].x; b += red[i][lane].y; }
-            if (p.db) p.db[c] = (float)a + (p.add_b ? p.db[c] : 0.f);
-            if (p.dw) p.dw[c] = (float)b + (p.add_w ? p.dw[c] : 0.f);
-        }
+    if ((int)blockIdx.x >= p.cap) {              // the last workgroups
+        if (!blockIdx.y) weight_sums(p, ((int)blockIdx.x - p.cap) * 64);
         return;
     }
     if ((int)blockIdx.x >= p.ntiles[1] || !p.out) return;
@@ -372,11 +380,282 @@ __global__ __launch_bounds__(NTH) void gn_bwd_apply_kernel(const NormArgs p) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------ documents that fit a workgroup's registers
+// One workgroup = one document x one slab of whole groups (64 bytes of a row or more where a few groups give that).  Its RT threads (512, two workgroups to
+// a CU; 1024 where 512 would keep more than 7 vectors each) load the slab into registers once (NR vectors of 16 bytes, all in flight together), reduce, and write the result: x is read once and nothing passes
+// through memory.  Slabs of one document are given to one XCD, whose L2 then serves the parts of a line that neighbouring slabs read.
+// Rows beyond NR * ny (a bound `longest` that is too small) are read from memory in both passes.
+constexpr int GAP_WGS = 64;
+
+struct Slab { int nslab, gs, sc; };              // slabs of a row, groups and channels of one
+
+__device__ __forceinline__ bool slab_of(const NormArgs& p, const Slab& sl, int& doc, int& c0) {
+    const int n = p.B * sl.nslab, per = (n + 7) / 8;                       // XCD = workgroup % 8: eight contiguous runs of (document, slab)
+    const int at = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+    if (((int)blockIdx.x >> 3) >= per || at >= n) return false;
+    doc = at / sl.nslab;
+    c0 = (at - doc * sl.nslab) * sl.sc;
+    return true;
+}
+template <typename T>
+__device__ __forceinline__ void zero_gaps(const NormArgs& p, int first) {  // the workgroups behind the slabs: rows of no document
+    for (int t = p.ntiles[0] + (int)blockIdx.x - first; t < p.ntiles[1]; t += GAP_WGS) {
+        const PackedTile tile = p.tiles[t];
+        zero_rows(reinterpret_cast<T*>(p.out) + (int64_t)tile.row0 * p.C, (int64_t)tile.n * p.C);
+    }
+}
+
+// sums of (a, b) over the threads of each group of the slab; every thread gets its group's.  group < 0: contributes nothing
+template <int RT>
+__device__ __forceinline__ double2 group_sums(double a, double b, int group, int gs, double2* part) {
+    // wave level first, group by group (a wave holds several groups), then the waves in LDS
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int g = 0; g < gs; ++g) {
+        const double u = lane_group_sum(group == g ? a : 0.0, 64), v = lane_group_sum(group == g ? b : 0.0, 64);
+        if (lane == 0) part[g * (RT / 64) + wave] = make_double2(u, v);
+    }
+    __syncthreads();
+    double2 r = make_double2(0.0, 0.0);
+    if (group >= 0)
+#pragma unroll
+        for (int w = 0; w < RT / 64; ++w) { const double2 v = part[group * (RT / 64) + w]; r.x += v.x; r.y += v.y; }
+    return r;
+}
+
+template <typename T, int V, int ACT, int NR, int RT>
+__global__ __launch_bounds__(RT, 4) void gn_resident_fwd_kernel(const NormArgs p, const Slab sl, int first_gap) {
+    extern __shared__ double2 part[];                                      // [gs][waves]
+    typedef typename PackedVec<T, V>::vec vec;
+    if ((int)blockIdx.x >= first_gap) { zero_gaps<T>(p, first_gap); return; }
+    int doc, c0;
+    if (!slab_of(p, sl, doc, c0)) return;
+    const int len = (int)p.len[doc];
+    if (len <= 0) return;
+    const int nx = sl.sc / V, ny = RT / nx, ry = threadIdx.x / nx, cx = threadIdx.x - ry * nx, cg = p.C / p.G;
+    const bool on = ry < ny;
+    const int64_t row0 = p.begin[doc];
+    const T* x = reinterpret_cast<const T*>(p.x) + row0 * p.ldx + c0 + cx * V;
+    T* y = reinterpret_cast<T*>(p.out) + row0 * p.C + c0 + cx * V;
+    vec keep[NR];
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+        const int r = k * ny + ry;
+        if (on && r < len) keep[k] = *reinterpret_cast<const vec*>(x + (int64_t)r * p.ldx);
+    }
+    double s = 0.0, q = 0.0;
+#pragma unroll
+    for (int k = 0; k < NR; ++k)
+        if (on && k * ny + ry < len)
+#pragma unroll
+            for (int i = 0; i < V; ++i) { const double d = (double)(float)keep[k][i]; s += d; q = fma(d, d, q); }
+    for (int r = NR * ny + ry; on && r < len; r += ny) {
+        float f[V];
+        PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx);
+#pragma unroll
+        for (int i = 0; i < V; ++i) { const double d = (double)f[i]; s += d; q = fma(d, d, q); }
+    }
+    const int g = on ? cx * V / cg : -1;
+    const double2 t = group_sums<RT>(s, q, g, sl.gs, part);
+    if (!on) return;
+    const double count = (double)len * (double)cg, md = t.x / count, var = fmax(t.y / count - md * md, 0.0);
+    const float m = (float)md, rs = (float)(1.0 / sqrt(var + (double)p.eps));
+    if (p.mean && ry == 0 && cx * V % cg == 0) {
+        p.mean[(int64_t)doc * p.G + c0 / cg + g] = m;
+        p.rstd[(int64_t)doc * p.G + c0 / cg + g] = rs;
+    }
+    float w[V], b[V];
+    PackedVec<float, V>::load(w, p.w + c0 + cx * V);
+    PackedVec<float, V>::load(b, p.b + c0 + cx * V);
+    auto apply = [&](float (&f)[V], int r) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = act_value<ACT, sizeof(T) == 4>(fmaf((f[i] - m) * rs, w[i], b[i]));
+        PackedVec<T, V>::store(y + (int64_t)r * p.C, f);
+    };
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+        const int r = k * ny + ry;
+        if (r < len) {
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = (float)keep[k][i];
+            apply(f, r);
+        }
+    }
+    for (int r = NR * ny + ry; r < len; r += ny) {
+        float f[V];
+        PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx);
+        apply(f, r);
+    }
+}
+
+template <typename T, int V, int ACT, int NR, int RT>
+__global__ __launch_bounds__(RT, 4) void gn_resident_bwd_kernel(const NormArgs p, const Slab sl, int first_gap) {
+    extern __shared__ double2 lds[];                                       // [gs][waves], then the channels' partial sums
+    typedef typename PackedVec<T, V>::vec vec;
+    if ((int)blockIdx.x >= first_gap) { if (p.out) zero_gaps<T>(p, first_gap); return; }
+    int doc, c0;
+    if (!slab_of(p, sl, doc, c0)) return;
+    const int len = (int)p.len[doc];
+    double2* sums = reinterpret_cast<double2*>(p.dsum) + (int64_t)doc * p.C + c0;
+    if (len <= 0) {
+        for (int c = threadIdx.x; c < sl.sc; c += RT) sums[c] = make_double2(0.0, 0.0);
+        return;
+    }
+    const int nx = sl.sc / V, ny = RT / nx, ry = threadIdx.x / nx, cx = threadIdx.x - ry * nx, cg = p.C / p.G;
+    const bool on = ry < ny;
+    const int64_t row0 = p.begin[doc];
+    const T* x = reinterpret_cast<const T*>(p.x) + row0 * p.ldx + c0 + cx * V;
+    const T* dy = reinterpret_cast<const T*>(p.dy) + row0 * p.lddy + c0 + cx * V;
+    vec kx[NR], kd[NR];
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+        const int r = k * ny + ry;
+        if (on && r < len) {
+            kx[k] = *reinterpret_cast<const vec*>(x + (int64_t)r * p.ldx);
+            kd[k] = *reinterpret_cast<const vec*>(dy + (int64_t)r * p.lddy);
+        }
+    }
+    const int g = on ? cx * V / cg : -1;
+    const int64_t stat = (int64_t)doc * p.G + c0 / cg + max(g, 0);
+    const float m = p.mean[stat], rs = p.rstd[stat];
+    float w[V], b[V], s[V], q[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { const int c = c0 + min(cx, nx - 1) * V + i; w[i] = p.w[c]; b[i] = p.b[c]; s[i] = 0.f; q[i] = 0.f; }
+    auto gather = [&](float xv, float dv, int i) {
+        const float hat = (xv - m) * rs, dz = dv * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i]));
+        s[i] += dz;
+        q[i] = fmaf(dz, hat, q[i]);
+    };
+#pragma unroll
+    for (int k = 0; k < NR; ++k)
+        if (on && k * ny + ry < len)
+#pragma unroll
+            for (int i = 0; i < V; ++i) gather((float)kx[k][i], (float)kd[k][i], i);
+    for (int r = NR * ny + ry; on && r < len; r += ny) {
+        float f[V], d[V];
+        PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx);
+        PackedVec<T, V>::load(d, dy + (int64_t)r * p.lddy);
+#pragma unroll
+        for (int i = 0; i < V; ++i) gather(f[i], d[i], i);
+    }
+    // channel sums: the threads' partials in LDS, added along the rows by RT / sc threads a channel, in two steps
+    double2* part = lds;
+    float2* stage = reinterpret_cast<float2*>(lds + sl.gs * (RT / 64));    // [ny][sc]
+    if (on)
+#pragma unroll
+        for (int i = 0; i < V; ++i) stage[ry * sl.sc + cx * V + i] = make_float2(s[i], q[i]);
+    __syncthreads();
+    const int np = RT / sl.sc, pr = threadIdx.x / sl.sc, pc = threadIdx.x - pr * sl.sc;
+    double sa = 0.0, sb = 0.0;
+    if (pr < np)
+        for (int r = pr; r < ny; r += np) { const float2 v = stage[r * sl.sc + pc]; sa += v.x; sb += v.y; }
+    __syncthreads();
+    double2* red = reinterpret_cast<double2*>(stage);                      // [np][sc]
+    if (pr < np) red[pr * sl.sc + pc] = make_double2(sa, sb);
+    __syncthreads();
+    double ga = 0.0, gb = 0.0;
+    int gg = -1;
+    if ((int)threadIdx.x < sl.sc) {
+        for (int i = 1; i < np; ++i) { const double2 v = red[i * sl.sc + threadIdx.x]; sa += v.x; sb += v.y; }
+        sums[threadIdx.x] = make_double2(sa, sb);
+        const double wc = (double)p.w[c0 + threadIdx.x];
+        ga = wc * sa; gb = wc * sb;
+        gg = (int)threadIdx.x / cg;
+    }
+    group_sums<RT>(ga, gb, gg, sl.gs, part);
+    if (!on || !p.out) return;
+    double2 t = make_double2(0.0, 0.0);
+#pragma unroll
+    for (int wv = 0; wv < RT / 64; ++wv) { const double2 v = part[g * (RT / 64) + wv]; t.x += v.x; t.y += v.y; }
+    const double inv = 1.0 / ((double)len * (double)cg);
+    const float c1 = (float)(t.x * inv), c2 = (float)(t.y * inv);
+    T* dx = reinterpret_cast<T*>(p.out) + row0 * p.C + c0 + cx * V;
+    auto apply = [&](float (&f)[V], const float (&d)[V], int r) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float hat = (f[i] - m) * rs;
+            const float gw = d[i] * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i])) * w[i];
+            f[i] = rs * (gw - c1 - hat * c2);
+        }
+        PackedVec<T, V>::store(dx + (int64_t)r * p.C, f);
+    };
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+        const int r = k * ny + ry;
+        if (r < len) {
+            float f[V], d[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) { f[i] = (float)kx[k][i]; d[i] = (float)kd[k][i]; }
+            apply(f, d, r);
+        }
+    }
+    for (int r = NR * ny + ry; r < len; r += ny) {
+        float f[V], d[V];
+        PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx);
+        PackedVec<T, V>::load(d, dy + (int64_t)r * p.lddy);
+        apply(f, d, r);
+    }
+}
+
+// dw, db: the documents' channel sums in their order, 64 channels a workgroup
+__global__ __launch_bounds__(NTH) void gn_weight_sums_kernel(const NormArgs p) { weight_sums(p, (int)blockIdx.x * 64); }
+
+// Slabs for documents of at most `longest` rows, vectors a thread keeps (0: such documents do not fit): whole groups, whole vectors in a group, the
+// narrowest slab with 64 bytes of a row, narrower ones where only they fit.
+int plan_slab(int64_t longest, int C, int G, int V, int RT, Slab& sl) {
+    const int cg = C / G, max_nr = 7;
+    if (cg % V || cg > RT) return 0;
+    int gs = 1;
+    while (gs < G && gs * cg * (16 / V) < 64) ++gs;
+    while (G % gs) ++gs;
+    for (;; gs = gs > 1 ? gs / 2 : 0) {
+        if (!gs) return 0;
+        if (G % gs) continue;
+        const int sc = gs * cg;
+        if (sc > RT) continue;
+        const int ny = RT / (sc / V);
+        const int64_t nr = cdiv(longest, ny);
+        if (nr <= max_nr) { sl.gs = gs; sl.sc = sc; sl.nslab = G / gs; return (int)nr; }
+    }
+}
+
 // parts of a tile: enough workgroups to fill the chip
 int parts(int64_t M) { return M >= 65536 ? 1 : M >= 16384 ? 2 : 4; }
 
+template <typename T, int V, int NR, int RT>
+void resident(const NormArgs& p, const Slab& sl, int act, bool backward, hipStream_t s) {
+    const int first_gap = (p.B * sl.nslab + 7) / 8 * 8;
+    const dim3 grid((unsigned)(first_gap + GAP_WGS));
+    const unsigned part = (unsigned)(sl.gs * (RT / 64) * sizeof(double2)), ny = (unsigned)(RT / (sl.sc / V));
+    const unsigned stage = (unsigned)(ny * sl.sc * sizeof(float2)), red = (unsigned)(RT / sl.sc * sl.sc * sizeof(double2));
+#define A(ACT_)                                                                                                                                 \
+    if (!backward) hipLaunchKernelGGL((gn_resident_fwd_kernel<T, V, ACT_, NR, RT>), grid, dim3(RT), part, s, p, sl, first_gap);                      \
+    else hipLaunchKernelGGL((gn_resident_bwd_kernel<T, V, ACT_, NR, RT>), grid, dim3(RT), part + (stage > red ? stage : red), s, p, sl, first_gap)
+    if (act == ACT_RELU) { A(ACT_RELU); } else if (act == ACT_GELU) { A(ACT_GELU); } else if (act == ACT_SILU) { A(ACT_SILU); } else { A(ACT_NONE); }
+#undef A
+    if (backward && (p.dw || p.db)) hipLaunchKernelGGL(gn_weight_sums_kernel, dim3((unsigned)cdiv(p.C, 64)), dim3(NTH), 0, s, p);
+}
+template <typename T, int V>
+bool try_resident(const NormArgs& p, int act, int64_t longest, bool backward, hipStream_t s) {
+    if constexpr (V == 1) return false;
+    else {
+        Slab sl;
+        if (!packed_aligned(p.w, 16) || !packed_aligned(p.b, 16)) return false;
+        int nr = plan_slab(longest, p.C, p.G, V, 512, sl);
+        if (nr == 0) {
+            nr = plan_slab(longest, p.C, p.G, V, 1024, sl);
+            if (nr == 0) return false;
+            if (nr <= 5) resident<T, V, 5, 1024>(p, sl, act, backward, s); else resident<T, V, 7, 1024>(p, sl, act, backward, s);
+        } else if (nr <= 2) resident<T, V, 2, 512>(p, sl, act, backward, s);
+        else if (nr <= 4) resident<T, V, 4, 512>(p, sl, act, backward, s);
+        else resident<T, V, 7, 512>(p, sl, act, backward, s);
+        return true;
+    }
+}
+
 template <typename T, int V>
 void forward(NormArgs p, int act, int64_t longest, hipStream_t s) {
+    if (try_resident<T, V>(p, act, longest, false, s)) return;
     const dim3 grid((unsigned)p.cap, (unsigned)p.sub);
     hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(NTH), (unsigned)((NTH * V + p.C) * sizeof(double2)), s, p);
     const bool direct = cdiv(longest, PACKED_TILE) * p.sub * p.G <= 2048;
@@ -389,7 +668,8 @@ void forward(NormArgs p, int act, int64_t longest, hipStream_t s) {
 }
 
 template <typename T, int V>
-void backward(NormArgs p, int act, hipStream_t s) {
+void backward(NormArgs p, int act, int64_t longest, hipStream_t s) {
+    if (try_resident<T, V>(p, act, longest, true, s)) return;
     const dim3 grid((unsigned)p.cap, (unsigned)p.sub), grid2((unsigned)(p.cap + cdiv(p.C, 64)), (unsigned)p.sub);
     const int cg = p.C / p.G, gchunk = cg >= 64 ? 1 : 64 / cg;
 #define A(ACT_)                                                                                                                                 \
@@ -448,8 +728,8 @@ extern "C" int osp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, i
     p.coef = reinterpret_cast<float*>(ws + B * C * 16 + slots * C * 8);
     const int V = bf16 ? 8 : 4;
     const bool wide = C % V == 0 && ldx % V == 0 && lddy % V == 0 && packed_aligned(x, 16) && packed_aligned(dy, 16) && packed_aligned(dx, 16);
-    if (bf16) { if (wide) backward<__bf16, 8>(p, (int)act, stream); else backward<__bf16, 1>(p, (int)act, stream); }
-    else { if (wide) backward<float, 4>(p, (int)act, stream); else backward<float, 1>(p, (int)act, stream); }
+    if (bf16) { if (wide) backward<__bf16, 8>(p, (int)act, longest, stream); else backward<__bf16, 1>(p, (int)act, longest, stream); }
+    else { if (wide) backward<float, 4>(p, (int)act, longest, stream); else backward<float, 1>(p, (int)act, longest, stream); }
     OSP_LAUNCH_CHECK();
     return OSP_OK;
 }

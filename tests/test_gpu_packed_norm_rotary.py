@@ -257,6 +257,26 @@ def test_group_norm_many_partials_take_the_separate_finish():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_group_norm_beyond_the_hosts_bound(dtype):
+    """documents longer than ``longest`` says: the rows a workgroup does not keep are read again, results agree with the right bound's
+    (the same sums in another order: 64-bit in the forward, chains of at most 900 rows in the backward)"""
+    from optispeech_amd import packed_ops as P
+    lengths, C, G = [900, 3, 400], 64, 4
+    M = sum(lengths)
+    x, g = randn(M, C, seed=1, dtype=dtype).requires_grad_(), randn(M, C, seed=2, dtype=dtype)
+    out = []
+    for longest in (900, 7):
+        w, b = torch.nn.Parameter(randn(C, seed=3)), torch.nn.Parameter(randn(C, seed=4))
+        rows = P.PackedRows.from_offsets(offsets(lengths), M, longest=longest)
+        y = P.group_norm(x, w, b, G, rows, 1e-5, "gelu")
+        out.append((y.detach(),) + torch.autograd.grad(y, (x,), g) + (w.grad, b.grad))
+    for i, (a, b) in enumerate(zip(*out)):
+        scale = a.double().abs().max().item()
+        assert float((a.double() - b.double()).abs().max()) <= (2 * half_eps(a.dtype) + 900 * U * (30 if i >= 2 else 1)) * scale
+
+
+@gpu
 def test_group_norm_strided_input_padded_rows_with_nan_and_frozen_weights():
     """x as a column slice of a wider tensor at an odd element, rows of no document hold NaN, weights want no gradient; parameter gradients of
     a second call add to the first one's"""
