@@ -40,7 +40,7 @@ struct Args {
     const int* ntiles;
     const int64_t* prefix;                              // per document or null
     const float* slopes;                                // per query head or null
-    int64_t Mq;
+    int64_t Mq, Mk, docs, qlongest, klongest;           // the last two: the host's bounds on a document, used to choose a kernel only
     int cap_tiles, Hq, Hk, G, D, causal;
     float scale, softcap;
 };
@@ -238,6 +238,19 @@ struct Score {
     __device__ __forceinline__ float derive(float c) const { return EXACT ? fmaf(-c, c, 1.f) : fmaf(-c, c, -c); }
     static constexpr float grad_scale = (MODE & CAP) && !EXACT ? 4.f : 1.f;
 };
+
+// host: too few tiles of 128 rows (of `heads` heads) to fill the chip: the waves of a workgroup share 32 rows instead of owning 32 each.  `path`: rows a
+// workgroup walks at most (times its heads).  Measured on both sides (causal, forward / dQ + dK + dV, us, wide -> split; n = tiles x heads):
+//   f32, width 64:   300 rows n = 90: 28 -> 18 / 95 -> 54, n = 182: 28 -> 29 / 98 -> 95, n = 360: 40 -> 46;  1000 rows n = 264: 86 -> 62 / 287 -> 211;
+//                    4000 rows n = 254: 293 -> 186 / 1048 -> 610, n = 1016: 579 -> 636
+//   bf16, width 128: 300 rows n = 22: 13.5 -> 10.5 / 38 -> 29, n = 90: 14.3 -> 13.5 / 41 -> 48;  1000 rows n = 66: 30 -> 17 / 89 -> 69, n = 264: 34 -> 35 /
+//                    98 -> 133;  4000 rows n = 248: 95 -> 72 / 307 -> 301, n = 1016: 164 -> 266
+static inline bool split_waves(int64_t rows, int64_t docs, int64_t heads, int64_t path, bool f32, bool narrow_limit) {
+    const int64_t n = (rows / PACKED_TILE + docs / 2) * heads;
+    if (f32) return n < (path >= 512 ? 384 : 192);
+    if (narrow_limit) return n < 72;                     // gradients of wide bf16 heads: the private tiles cost occupancy
+    return n < (path >= 2048 ? 384 : 128);
+}
 
 // host: a tile's rows fit a buffer descriptor, and a row reaches no further than the next
 static inline bool row_stride_ok(int64_t stride, int64_t D, int64_t bf16) { return stride >= D && stride * (bf16 ? 2 : 4) < (int64_t)1 << 24; }

@@ -292,7 +292,8 @@ def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):
              D, scale, softcap, causal)
     elif M:
         call("osp_packed_attention_fwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, rest,
-             lse, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, prefix, slopes, M, H, S, D, scale, softcap, causal)
+             lse, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, prefix, slopes, rows.docs, keys.longest,
+             M, H, S, D, scale, softcap, causal)
     return q, k, v, o, rest, lse
 
 
@@ -316,7 +317,8 @@ class PackedAttentionFn(torch.autograd.Function):
             delta = torch.empty_like(lse)
             call("osp_packed_attention_bwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), o, rest, lse, do,
                  do.stride(0), do.stride(1), int(q.dtype == torch.bfloat16), dq, dk, dv, delta, rows.begin, rows.length, rows.tiles, rows.ntiles,
-                 rows.cap, keys.begin, keys.length, keys.tiles, keys.ntiles, keys.cap, prefix, slopes, M, H, S, D, scale, softcap, causal)
+                 rows.cap, keys.begin, keys.length, keys.tiles, keys.ntiles, keys.cap, prefix, slopes, rows.docs, rows.longest, keys.longest, M, Mk, H, S, D,
+                 scale, softcap, causal)
         else:
             dq.zero_(), dk.zero_(), dv.zero_()
         return dq, dk, dv, None, None, None, None, None, None, None
