@@ -7,8 +7,8 @@
 // position"); the product's nearest quarter turn is taken off in 64 bits and the rest, |r| <= 1/8 turn, goes to f32: an angle of at most
 // pi / 4 whose rounding is 2^-25 of it.  sin and cos of it are Taylor sums (degree 9 and 10; the first term left out is below 2e-9).
 //
-// Bound: HBM.  A thread owns V pairs of one row and keeps their cos / sin in registers over all heads of q and k, so the 64-bit work is done
-// once per row and not once per head; all its loads and stores are 16 bytes where alignment allows.
+// Bound: HBM.  The 64-bit work is done once per row and pair, into LDS, and serves all heads of q and k; the heads are then walked in the order of memory
+// with accesses of 16 bytes where alignment allows.
 #include "packed_common.h"
 
 namespace {
@@ -42,71 +42,81 @@ __device__ __forceinline__ void turn_sincos(double t, float& s, float& c) {
     c = ((k + 1) & 2) ? -c1 : c1;
 }
 
-// V pairs per slot.  Slots of a row: R / 2 / V that turn, then (D - R) / (2 V) rounded up that copy (2 V channels each, the last one short).
+// V pairs per slot.  First the workgroup's rows' cos and sin go to LDS (rows x R / 2 pairs, mag and the direction's sign included); then its threads walk
+// (row, head, slot) in the order of memory, BATCH vectors in flight each.
 template <typename TI, typename TO, int V, bool HALF>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs p, int rows_per_wg) {
-    const int nt = p.ntiles[1];
-    if ((int)blockIdx.x >= nt) return;
+    extern __shared__ float2 turn_l[];
+    constexpr int BATCH = 4, W = HALF ? V : 2 * V;                 // channels of one access
     const PackedTile tile = p.tiles[blockIdx.x];
-    const int turning = p.R / 2 / V, copying = (p.D - p.R + 2 * V - 1) / (2 * V), slots = turning + copying;
-    const int r_lo = blockIdx.y * rows_per_wg, r_hi = min(tile.n, r_lo + rows_per_wg);
-    if (r_lo >= r_hi) return;
-    const int total = (r_hi - r_lo) * slots;
+    if ((int)blockIdx.x >= p.ntiles[1]) return;
+    const int r_lo = blockIdx.y * rows_per_wg, n = min(tile.n - r_lo, rows_per_wg), tid = threadIdx.x;
+    if (n <= 0) return;
+    const int64_t row0 = (int64_t)tile.row0 + r_lo;
     if (tile.doc < 0) {                                           // rows of no document: zeros
         for (int which = 0; which < 2; ++which) {
-            TO* y = reinterpret_cast<TO*>(p.y[which]) + (int64_t)(tile.row0 + r_lo) * p.heads[which] * p.D;
-            const int64_t n = (int64_t)(r_hi - r_lo) * p.heads[which] * p.D;
-            for (int64_t i = threadIdx.x; i < n; i += 256) y[i] = (TO)0.f;
+            TO* y = reinterpret_cast<TO*>(p.y[which]) + row0 * p.heads[which] * p.D;
+            const int64_t total = (int64_t)n * p.heads[which] * p.D;
+            for (int64_t i = tid; i < total; i += 256) y[i] = (TO)0.f;
         }
         return;
     }
-    const int64_t first = p.first ? p.first[tile.doc] : 0;
-    for (int u = threadIdx.x; u < total; u += 256) {
-        const int r = r_lo + u / slots, slot = u % slots;
-        const int64_t row = (int64_t)tile.row0 + r;
-        if (slot < turning) {
-            const double pos = (double)(first + tile.i0 + r);
-            float s[V], c[V];
+    const int half = p.R / 2;
+    const int64_t pos0 = (p.first ? p.first[tile.doc] : 0) + tile.i0 + r_lo;
+    for (int u = tid; u < n * half; u += 256) {
+        const int r = u / half;
+        float s, c;
+        turn_sincos((double)(pos0 + r) * p.turns[u - r * half], s, c);
+        turn_l[u] = make_float2(c * p.mag, p.inverse ? -s * p.mag : s * p.mag);
+    }
+    __syncthreads();
+    const int turning = half / V, lanes = min(turning, 256), step = 256 / lanes, slot0 = tid % lanes, item0 = tid / lanes;
+    for (int which = 0; which < 2; ++which) {
+        const int heads = p.heads[which], items = n * heads;
+        const TI* x = reinterpret_cast<const TI*>(p.x[which]) + row0 * p.xr[which];
+        TO* y = reinterpret_cast<TO*>(p.y[which]) + row0 * heads * p.D;
+        for (int slot = slot0; slot < turning && item0 < step; slot += lanes) {
+            const int at = slot * W;
+            for (int item = item0; item < items; item += BATCH * step) {
+                float a[BATCH][W], b[BATCH][HALF ? W : 1];
+                int rr[BATCH];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                turn_sincos(pos * p.turns[slot * V + i], s[i], c[i]);
-                s[i] *= p.inverse ? -p.mag : p.mag;
-                c[i] *= p.mag;
-            }
-            for (int which = 0; which < 2; ++which) {
-                const TI* x = reinterpret_cast<const TI*>(p.x[which]) + row * p.xr[which];
-                TO* y = reinterpret_cast<TO*>(p.y[which]) + row * p.heads[which] * p.D;
-#pragma unroll 4
-                for (int h = 0; h < p.heads[which]; ++h) {
-                    if constexpr (HALF) {
-                        const int at = slot * V;
-                        float a[V], b[V], ya[V], yb[V];
-                        PackedVec<TI, V>::load(a, x + h * p.xh[which] + at);
-                        PackedVec<TI, V>::load(b, x + h * p.xh[which] + p.R / 2 + at);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) { ya[i] = a[i] * c[i] - b[i] * s[i]; yb[i] = a[i] * s[i] + b[i] * c[i]; }
-                        PackedVec<TO, V>::store(y + h * p.D + at, ya);
-                        PackedVec<TO, V>::store(y + h * p.D + p.R / 2 + at, yb);
-                    } else {
-                        const int at = slot * 2 * V;
-                        float a[2 * V], b[2 * V];
-                        PackedVec<TI, 2 * V>::load(a, x + h * p.xh[which] + at);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            b[2 * i] = a[2 * i] * c[i] - a[2 * i + 1] * s[i];
-                            b[2 * i + 1] = a[2 * i] * s[i] + a[2 * i + 1] * c[i];
-                        }
-                        PackedVec<TO, 2 * V>::store(y + h * p.D + at, b);
+                for (int j = 0; j < BATCH; ++j) {
+                    const int it = item + j * step;
+                    rr[j] = it / heads;
+                    if (it < items) {
+                        const TI* src = x + rr[j] * p.xr[which] + (it - rr[j] * heads) * p.xh[which] + at;
+                        PackedVec<TI, W>::load(a[j], src);
+                        if constexpr (HALF) PackedVec<TI, W>::load(b[j], src + half);
                     }
                 }
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const int it = item + j * step;
+                    if (it >= items) continue;
+                    const float2* cs = turn_l + rr[j] * half + slot * V;
+                    TO* dst = y + (int64_t)it * p.D + at;
+                    float u[W], w[HALF ? W : 1];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float2 t = cs[i];
+                        if constexpr (HALF) { u[i] = a[j][i] * t.x - b[j][i] * t.y; w[i] = a[j][i] * t.y + b[j][i] * t.x; }
+                        else { u[2 * i] = a[j][2 * i] * t.x - a[j][2 * i + 1] * t.y; u[2 * i + 1] = a[j][2 * i] * t.y + a[j][2 * i + 1] * t.x; }
+                    }
+                    PackedVec<TO, W>::store(dst, u);
+                    if constexpr (HALF) PackedVec<TO, W>::store(dst + half, w);
+                }
             }
-        } else {
-            const int at = p.R + (slot - turning) * 2 * V, n = min(2 * V, p.D - at);
-            for (int which = 0; which < 2; ++which) {
-                const TI* x = reinterpret_cast<const TI*>(p.x[which]) + row * p.xr[which] + at;
-                TO* y = reinterpret_cast<TO*>(p.y[which]) + row * p.heads[which] * p.D + at;
-                for (int h = 0; h < p.heads[which]; ++h)
-                    for (int i = 0; i < n; ++i) y[h * p.D + i] = (TO)(float)x[h * p.xh[which] + i];
+        }
+        const int rest = p.D - p.R;                               // the remaining channels pass
+        if (rest) {
+            const int per = V > 1 && rest % W == 0 ? W : 1, chunks = rest / per;
+            for (int u = tid; u < items * chunks; u += 256) {
+                const int it = u / chunks, c = p.R + (u - it * chunks) * per, r = it / heads;
+                const TI* src = x + r * p.xr[which] + (it - r * heads) * p.xh[which] + c;
+                TO* dst = y + (int64_t)it * p.D + c;
+                if (per > 1) { float f[W]; PackedVec<TI, W>::load(f, src); PackedVec<TO, W>::store(dst, f); }
+                else *dst = (TO)(float)*src;
             }
         }
     }
@@ -116,8 +126,8 @@ template <typename TI, typename TO, bool HALF>
 void launch(const RotaryArgs& p, int V, dim3 grid, int rows_per_wg, hipStream_t stream) {
     // V pairs: the widest accesses of 16 bytes that alignment and R allow (one pair otherwise)
     constexpr int VW = HALF ? (sizeof(TI) == 2 ? 8 : 4) : (sizeof(TI) == 2 ? 4 : 2);
-    if (V > 1) hipLaunchKernelGGL((rotary_kernel<TI, TO, VW, HALF>), grid, dim3(256), 0, stream, p, rows_per_wg);
-    else hipLaunchKernelGGL((rotary_kernel<TI, TO, 1, HALF>), grid, dim3(256), 0, stream, p, rows_per_wg);
+    if (V > 1) hipLaunchKernelGGL((rotary_kernel<TI, TO, VW, HALF>), grid, dim3(256), (unsigned)(rows_per_wg * p.R * 4), stream, p, rows_per_wg);
+    else hipLaunchKernelGGL((rotary_kernel<TI, TO, 1, HALF>), grid, dim3(256), (unsigned)(rows_per_wg * p.R * 4), stream, p, rows_per_wg);
 }
 
 }  // namespace
@@ -143,10 +153,9 @@ extern "C" int osp_rotary(const void* q, int64_t q_row, int64_t q_head, const vo
     for (int w = 0; w < 2; ++w)
         wide = wide && packed_aligned(p.x[w], ib) && packed_aligned(p.y[w], ob) && p.xr[w] % run == 0 && p.xh[w] % run == 0;
     const int V = wide ? VW : 1;
-    const int slots = (int)(R / 2 / V + (D - R + 2 * V - 1) / (2 * V));
-    // rows of a workgroup: about one slot per thread
-    int rows = 256 / slots;
-    rows = rows < 1 ? 1 : rows > PACKED_TILE ? PACKED_TILE : rows;
+    // rows of a workgroup: 16, fewer where their cos and sin would take more than 32 KB
+    int rows = (int)(8192 / R);
+    rows = rows < 1 ? 1 : rows > 16 ? 16 : rows;
     const dim3 grid((unsigned)cap, (unsigned)cdiv(PACKED_TILE, rows));
     if (in_bf16 && out_bf16) { if (interleaved) launch<__bf16, __bf16, false>(p, V, grid, rows, stream); else launch<__bf16, __bf16, true>(p, V, grid, rows, stream); }
     else if (in_bf16) { if (interleaved) launch<__bf16, float, false>(p, V, grid, rows, stream); else launch<__bf16, float, true>(p, V, grid, rows, stream); }
