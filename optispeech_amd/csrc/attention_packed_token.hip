@@ -130,33 +130,56 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_token
     }
 }
 
-// joins the splits of every query row and head; rows of no document become zeros
+// joins the splits of every query row and head; rows of no document become zeros.  D / 4 threads hold a row, groups of them take the splits in turn (their
+// loads are in flight together) and meet in LDS, in the order of the groups.
 template <typename T>
 __global__ __launch_bounds__(256) void packed_attn_join_kernel(const Args p, int chunk, int nsplit, const float* __restrict__ po, const float* __restrict__ pm) {
-    if ((int)blockIdx.x >= p.ntiles[1]) return;
+    __shared__ float4 red_a[256];
+    __shared__ float2 red_m[256];
     const PackedTile tile = p.tiles[blockIdx.x];
-    const int h = blockIdx.y, quads = p.D / 4;
+    if ((int)blockIdx.x >= p.ntiles[1]) return;
+    const int h = blockIdx.y, quads = p.D / 4, groups = 256 / quads, g = threadIdx.x / quads, d = (threadIdx.x - g * quads) * 4;
     int n = 0;
     if (tile.doc >= 0) {
         const int klen = (int)p.klen[tile.doc];
         n = max(1, min(nsplit, (klen + chunk - 1) / chunk));
     }
-    for (int u = threadIdx.x; u < tile.n * quads; u += 256) {
-        const int r = u / quads, d = (u - r * quads) * 4;
-        const int64_t row = (int64_t)tile.row0 + r, slot0 = row * p.Hq + h, step = p.Mq * p.Hq;
-        float m = NONE, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < n; ++s) m = fmaxf(m, pm[(slot0 + s * step) * 2]);
+    const int64_t step = p.Mq * p.Hq;
+    for (int r = 0; r < tile.n; ++r) {
+        const int64_t slot0 = ((int64_t)tile.row0 + r) * p.Hq + h;
+        float m = NONE, l = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (g < groups) {
 #pragma unroll 4
-        for (int s = 0; s < n; ++s) {
-            const float2 x = *reinterpret_cast<const float2*>(pm + (slot0 + s * step) * 2);
-            const float4 y = *reinterpret_cast<const float4*>(po + (slot0 + s * step) * p.D + d);
-            const float f = __builtin_amdgcn_exp2f(x.x - m);
-            l = fmaf(x.y, f, l);
-            a[0] = fmaf(y.x, f, a[0]); a[1] = fmaf(y.y, f, a[1]); a[2] = fmaf(y.z, f, a[2]); a[3] = fmaf(y.w, f, a[3]);
+            for (int s = g; s < n; s += groups) {
+                const float2 x = *reinterpret_cast<const float2*>(pm + (slot0 + s * step) * 2);
+                const float4 y = *reinterpret_cast<const float4*>(po + (slot0 + s * step) * p.D + d);
+                const float mn = fmaxf(m, x.x), fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(x.x - mn);
+                m = mn;
+                l = l * fo + x.y * fn;
+                a = make_float4(a.x * fo + y.x * fn, a.y * fo + y.y * fn, a.z * fo + y.z * fn, a.w * fo + y.w * fn);
+            }
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const float o[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
-        PackedVec<T, 4>::store(reinterpret_cast<T*>(p.out) + slot0 * p.D + d, o);
+        red_a[threadIdx.x] = a;
+        red_m[threadIdx.x] = make_float2(m, l);
+        __syncthreads();
+        if (g == 0) {
+            const int live = min(groups, max(n, 1));
+            for (int i = 1; i < live; ++i) m = fmaxf(m, red_m[i * quads + threadIdx.x].x);
+            l = 0.f;
+            a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < live; ++i) {
+                const float2 x = red_m[i * quads + threadIdx.x];
+                const float4 y = red_a[i * quads + threadIdx.x];
+                const float f = __builtin_amdgcn_exp2f(x.x - m);
+                l = fmaf(x.y, f, l);
+                a = make_float4(fmaf(y.x, f, a.x), fmaf(y.y, f, a.y), fmaf(y.z, f, a.z), fmaf(y.w, f, a.w));
+            }
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const float o[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+            PackedVec<T, 4>::store(reinterpret_cast<T*>(p.out) + slot0 * p.D + d, o);
+        }
+        __syncthreads();
     }
 }
 
