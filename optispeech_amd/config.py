@@ -37,6 +37,9 @@ class ModelConfig:
     tf_units: int = 1024
     tf_blocks: int = 4
     tf_dropout: float = 0.2
+    #: Transformer / Conformer backbones: None = the reference's attention; a dict = options of the packed attention (model/packed.py), e.g.
+    #: dict(rotary={}, softcap=30.0); the Conformer then normalises its convolutions with group norm
+    packed_attention: dict = None
     dur: tuple = (2, 384, 3, 0.1)                         # layers, channels, kernel, dropout
     pitch: tuple = (5, 256, 5, 0.5)
     energy: tuple = (2, 384, 3, 0.5)
@@ -78,6 +81,8 @@ def _backbones(c):
         from .model.transformer import Transformer
         tf = partial(Transformer, attention_heads=c.tf_heads, linear_units=c.tf_units, num_blocks=c.tf_blocks,
                      dropout_rate=c.tf_dropout, positional_dropout_rate=c.tf_dropout, attention_dropout_rate=c.tf_dropout)
+        if c.packed_attention is not None:
+            tf = partial(tf, selfattention_layer_type="packed", packed=c.packed_attention, attention_dropout_rate=0.0)
         return tf, tf
     if c.backbone == "lightspeech":
         # configs/model/generator/{encoder,decoder}/lightspeech_transformer.yaml
@@ -90,6 +95,8 @@ def _backbones(c):
         from .model.conformer import Conformer
         kw = dict(attention_heads=2, linear_units=1024, num_blocks=4, dropout_rate=0.2, positional_dropout_rate=0.2,
                   attention_dropout_rate=0.2)
+        if c.packed_attention is not None:
+            kw.update(selfattention_layer_type="packed", packed=c.packed_attention, attention_dropout_rate=0.0)
         return partial(Conformer, cnn_module_kernel=7, **kw), partial(Conformer, cnn_module_kernel=31, **kw)
     if c.backbone == "leanspeech":
         # configs/model/generator/{encoder,decoder}/leanspeech.yaml

@@ -117,18 +117,26 @@ class _DepthwiseConv(RefSchemaModule):
 class ConvolutionModule(nn.Module):
     """_conformer/convolution.py:13-78: pointwise (C -> 2C) -> GLU -> depthwise k -> BatchNorm -> swish -> pointwise."""
 
-    def __init__(self, channels, kernel_size):
+    def __init__(self, channels, kernel_size, norm_groups=None):
+        """norm_groups: group norm over each utterance's frames in the place of BatchNorm, its swish fused"""
         super().__init__()
         assert (kernel_size - 1) % 2 == 0
         self.pointwise_conv1 = _Conv1dK1(channels, 2 * channels)
         self.depthwise_conv = _DepthwiseConv(channels, kernel_size)
-        self.norm = _BatchNorm1d(channels)
+        if norm_groups is None:
+            self.norm = _BatchNorm1d(channels)
+        else:
+            from .packed import PackedGroupNorm
+            self.norm = PackedGroupNorm(norm_groups, channels, act="silu")
+        self.norm_groups = norm_groups
         self.pointwise_conv2 = _Conv1dK1(channels, channels)
 
-    def forward(self, x):
+    def forward(self, x, rows=None, valid=None):
         C = x.shape[-1]
         u = self.pointwise_conv1(x)
         u = u[..., :C] * torch.sigmoid(u[..., C:])                                               # GLU over the channel pairs
+        if self.norm_groups is not None:                          # padded frames stay out of the convolution and of the statistics
+            return self.pointwise_conv2(self.norm(self.depthwise_conv((u * valid).contiguous()), rows))
         u = self.norm(self.depthwise_conv(u.contiguous()))
         return self.pointwise_conv2(u * torch.sigmoid(u))                                        # swish
 
@@ -150,10 +158,14 @@ class EncoderLayer(nn.Module):
             y = y * scale
         return ops.dropout_add(y, self.dropout_rate, self.training, self._s[i], res=x)
 
-    def forward(self, x, pos_emb, klen):
+    def forward(self, x, pos_emb, klen, rows=None, valid=None):
         x = self._res(x, self.feed_forward_macaron(self.norm_ff_macaron(x)), 0, 0.5)
-        x = self._res(x, self.self_attn(self.norm_mha(x), pos_emb, klen), 1)
-        x = self._res(x, self.conv_module(self.norm_conv(x)), 2)
+        if rows is None:
+            x = self._res(x, self.self_attn(self.norm_mha(x), pos_emb, klen), 1)
+            x = self._res(x, self.conv_module(self.norm_conv(x)), 2)
+        else:
+            x = self._res(x, self.self_attn(self.norm_mha(x), rows), 1)
+            x = self._res(x, self.conv_module(self.norm_conv(x), rows, valid), 2)
         x = self._res(x, self.feed_forward(self.norm_ff(x)), 3, 0.5)
         return self.norm_final(x)
 
@@ -162,14 +174,20 @@ class Encoder(nn.Module):
     """_conformer/encoder.py (input_layer None, rel_pos): x * sqrt(d) -> dropout; pos_emb -> dropout; blocks; after_norm."""
 
     def __init__(self, attention_dim, attention_heads, linear_units, num_blocks, dropout_rate, positional_dropout_rate,
-                 attention_dropout_rate, cnn_module_kernel):
+                 attention_dropout_rate, cnn_module_kernel, packed=None, norm_groups=None):
         super().__init__()
-        self.d, self.pos_drop = attention_dim, positional_dropout_rate
+        self.d, self.pos_drop, self.packed = attention_dim, positional_dropout_rate, packed is not None
+
+        def attention():
+            if packed is None:
+                return RelPositionMultiHeadedAttention(attention_heads, attention_dim, attention_dropout_rate)
+            from .packed import PackedSelfAttention
+            return PackedSelfAttention(attention_heads, attention_dim, **packed)
         self.encoders = nn.ModuleList([
-            EncoderLayer(attention_dim, RelPositionMultiHeadedAttention(attention_heads, attention_dim, attention_dropout_rate),
+            EncoderLayer(attention_dim, attention(),
                          MultiLayeredConv1d(attention_dim, linear_units, 1, dropout_rate),
                          MultiLayeredConv1d(attention_dim, linear_units, 1, dropout_rate),
-                         ConvolutionModule(attention_dim, cnn_module_kernel), dropout_rate)
+                         ConvolutionModule(attention_dim, cnn_module_kernel, norm_groups), dropout_rate)
             for _ in range(num_blocks)])
         self.after_norm = FinalNorm(attention_dim, 1e-12)
         self._s = [rng.new_stream(), rng.new_stream()]
@@ -177,6 +195,13 @@ class Encoder(nn.Module):
     def forward(self, xs, klen):
         T = xs.shape[1]
         xs = ops.dropout_add(xs * math.sqrt(self.d), self.pos_drop, self.training, self._s[0])
+        if self.packed:
+            from ..packed_ops import PackedRows
+            rows = PackedRows.from_padded(klen, T)
+            valid = (torch.arange(T, device=xs.device)[None] < klen[:, None])[:, :, None].to(xs.dtype)
+            for layer in self.encoders:
+                xs = layer(xs, None, None, rows, valid)
+            return self.after_norm(xs)
         pos = rel_positions(T, self.d, xs.device)
         if self.training and self.pos_drop > 0.0 and (2 * T - 1) * self.d % 4 == 0:
             pos = ops.dropout_add(pos, self.pos_drop, True, self._s[1])
@@ -186,20 +211,28 @@ class Encoder(nn.Module):
 
 
 class Conformer(nn.Module):
-    """generator/modules/conformer.py:9-28.  forward(x (B, T, C), padding_mask (B, T) True = pad) -> (B, T, C)."""
+    """generator/modules/conformer.py:9-28.  forward(x (B, T, C), padding_mask (B, T) True = pad) -> (B, T, C).
+
+    selfattention_layer_type="packed": the attention of model/packed.py with the keyword arguments ``packed`` (rotary positions unless it says
+    otherwise), attention_dropout_rate 0, and group norm over ``cnn_module_norm_groups`` groups of each utterance's own frames in the convolution
+    module: an utterance's frames do not depend on the padding or the other utterances of its batch."""
 
     def __init__(self, dim, attention_heads=2, linear_units=1024, num_blocks=4, dropout_rate=0.2, positional_dropout_rate=0.2,
                  attention_dropout_rate=0.2, normalize_before=True, concat_after=False, positionwise_layer_type="conv1d",
                  positionwise_conv_kernel_size=1, macaron_style=True, pos_enc_layer_type="rel_pos",
                  selfattention_layer_type="rel_selfattn", activation_type="swish", use_cnn_module=True, cnn_module_kernel=7,
-                 zero_triu=False, init_type="xavier_uniform", **unused):
+                 zero_triu=False, init_type="xavier_uniform", packed=None, cnn_module_norm_groups=8, **unused):
         super().__init__()
         assert normalize_before and not concat_after and positionwise_layer_type == "conv1d" and positionwise_conv_kernel_size == 1
-        assert macaron_style and pos_enc_layer_type == "rel_pos" and selfattention_layer_type == "rel_selfattn"
+        is_packed = selfattention_layer_type == "packed"
+        assert is_packed or packed is None, "`packed` holds options of selfattention_layer_type='packed'"
+        assert not is_packed or attention_dropout_rate == 0.0, "the packed attention has no dropout on its probabilities"
+        assert macaron_style and (is_packed or (pos_enc_layer_type == "rel_pos" and selfattention_layer_type == "rel_selfattn"))
         assert activation_type == "swish" and use_cnn_module and not zero_triu, \
             "only the configuration of configs/model/generator/*/conformer.yaml is built"
         self.conformer = Encoder(dim, attention_heads, linear_units, num_blocks, dropout_rate, positional_dropout_rate,
-                                 attention_dropout_rate, cnn_module_kernel)
+                                 attention_dropout_rate, cnn_module_kernel, dict({"rotary": {}}, **(packed or {})) if is_packed else None,
+                                 cnn_module_norm_groups if is_packed else None)
 
     def forward(self, x, padding_mask):
         klen = (~padding_mask).sum(1).to(torch.int64)

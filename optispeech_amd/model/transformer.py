@@ -13,7 +13,7 @@ import math
 import torch
 from torch import nn
 
-from .. import ops, rng
+from .. import ops, precision, rng
 from .base import RefSchemaModule, conv_to_native, conv_to_ref
 from .modules import FinalNorm
 
@@ -129,8 +129,8 @@ class EncoderLayer(nn.Module):
         self.dropout_rate = dropout_rate
         self._s1, self._s2 = rng.new_stream(), rng.new_stream()
 
-    def forward(self, x, klen):
-        x = _dropout(self.self_attn(self.norm1(x), klen), self.dropout_rate, self.training, self._s1, res=x)
+    def forward(self, x, klen, *cache):
+        x = _dropout(self.self_attn(self.norm1(x), klen, *cache), self.dropout_rate, self.training, self._s1, res=x)
         return _dropout(self.feed_forward(self.norm2(x)), self.dropout_rate, self.training, self._s2, res=x)
 
 
@@ -138,36 +138,55 @@ class Encoder(nn.Module):
     """_transformer/encoder.py (input_layer None, pos_enc_class ScaledPositionalEncoding): embed -> encoders -> after_norm."""
 
     def __init__(self, attention_dim, attention_heads, linear_units, num_blocks, dropout_rate, positional_dropout_rate,
-                 attention_dropout_rate):
+                 attention_dropout_rate, packed=None):
         super().__init__()
-        self.embed = nn.Sequential(ScaledPositionalEncoding(attention_dim, positional_dropout_rate))
+        if packed is None or packed.get("rotary") is None:
+            self.embed = nn.Sequential(ScaledPositionalEncoding(attention_dim, positional_dropout_rate))
+        else:                                                     # positions enter with the queries and keys
+            self.embed = None
+
+        def attention():
+            if packed is None:
+                return MultiHeadedAttention(attention_heads, attention_dim, attention_dropout_rate)
+            from .packed import PackedSelfAttention
+            return PackedSelfAttention(attention_heads, attention_dim, **packed)
         self.encoders = nn.ModuleList([
-            EncoderLayer(attention_dim, MultiHeadedAttention(attention_heads, attention_dim, attention_dropout_rate),
-                         MultiLayeredConv1d(attention_dim, linear_units, 1, dropout_rate), dropout_rate)
+            EncoderLayer(attention_dim, attention(), MultiLayeredConv1d(attention_dim, linear_units, 1, dropout_rate), dropout_rate)
             for _ in range(num_blocks)])
         self.after_norm = FinalNorm(attention_dim, 1e-12)
 
     def forward(self, xs, klen):
-        xs = self.embed(xs)
+        """klen: the valid-key counts, or the PackedRows of the frames where the attention is the packed one"""
+        if self.embed is not None:
+            xs = self.embed(xs)
         for layer in self.encoders:
             xs = layer(xs, klen)
         return self.after_norm(xs)
 
 
 class Transformer(nn.Module):
-    """generator/modules/transformer.py:9-27.  forward(x (B, T, C), padding_mask (B, T) True = pad) -> (B, T, C)."""
+    """generator/modules/transformer.py:9-27.  forward(x (B, T, C), padding_mask (B, T) True = pad) -> (B, T, C).
+
+    selfattention_layer_type="packed": the attention of model/packed.py with the keyword arguments ``packed`` (rotary positions, capped scores, distance
+    penalties, causal masks, shared key heads), attention_dropout_rate 0.  Then ``forward_packed`` takes utterances packed behind each other, and
+    a causal backbone with rotary positions runs frame by frame (``start_stream``, ``stream``)."""
 
     def __init__(self, dim, attention_heads=2, linear_units=1024, num_blocks=4, dropout_rate=0.2, positional_dropout_rate=0.2,
                  attention_dropout_rate=0.2, normalize_before=True, concat_after=False, positionwise_layer_type="conv1d",
-                 positionwise_conv_kernel_size=1, use_scaled_pos_enc=True, init_alpha=1.0, init_type="xavier_uniform", **unused):
+                 positionwise_conv_kernel_size=1, use_scaled_pos_enc=True, init_alpha=1.0, init_type="xavier_uniform",
+                 selfattention_layer_type="selfattn", packed=None, **unused):
         super().__init__()
+        self.packed = selfattention_layer_type == "packed"
+        assert self.packed or packed is None, "`packed` holds options of selfattention_layer_type='packed'"
+        assert not self.packed or attention_dropout_rate == 0.0, "the packed attention has no dropout on its probabilities"
         assert normalize_before and not concat_after and positionwise_layer_type == "conv1d" and use_scaled_pos_enc, \
             "only the configuration of configs/model/generator/*/transformer.yaml is built"
         assert positionwise_conv_kernel_size == 1
         self.transformer = Encoder(dim, attention_heads, linear_units, num_blocks, dropout_rate, positional_dropout_rate,
-                                   attention_dropout_rate)
-        with torch.no_grad():
-            self.transformer.embed[-1].alpha.fill_(init_alpha)
+                                   attention_dropout_rate, dict(packed or {}) if self.packed else None)
+        if self.transformer.embed is not None:
+            with torch.no_grad():
+                self.transformer.embed[-1].alpha.fill_(init_alpha)
 
     def forward(self, x, padding_mask):
         # mask = ~padding_mask (prefix-valid, as sequence_mask builds it): the valid-key counts are the lengths the mask was built
@@ -181,4 +200,31 @@ class Transformer(nn.Module):
             klen = tag[1]
         else:
             klen = (~padding_mask).sum(1).to(torch.int64)
+        if self.packed:
+            from ..packed_ops import PackedRows
+            return self.transformer(x, PackedRows.from_padded(klen.contiguous(), x.shape[1]))
         return self.transformer(x, klen)
+
+    def forward_packed(self, x, rows):
+        """x (M, C): the documents of ``rows`` (packed_ops.PackedRows) behind each other -> (M, C); every utterance gets what it gets alone"""
+        assert self.packed and self.transformer.embed is None, "packed utterances need selfattention_layer_type='packed' with rotary positions"
+        return self.transformer(x[None], rows)[0]
+
+    def start_stream(self, streams, capacity):
+        """Keys and values of ``streams`` streams of at most ``capacity`` frames"""
+        att = [layer.self_attn for layer in self.transformer.encoders]
+        assert self.packed and self.transformer.embed is None and all(a.causal for a in att), \
+            "streams need selfattention_layer_type='packed', rotary positions and a causal mask"
+        from .packed import FrameCache
+        return FrameCache(len(att), streams, capacity, att[0].s, att[0].d_k, self.transformer.after_norm.weight.device,
+                          torch.bfloat16 if precision.is_bf16() else torch.float32)
+
+    @torch.no_grad()
+    def stream(self, x, cache):
+        """x (streams, n, C): the next n frames of every stream -> their outputs, equal to the causal forward over all frames so far"""
+        assert not self.training, "streams run in eval mode"
+        rows = cache.begin(x.shape[1])
+        for i, layer in enumerate(self.transformer.encoders):
+            x = layer(x, rows, cache, i)
+        cache.end(rows.longest)
+        return self.transformer.after_norm(x)
