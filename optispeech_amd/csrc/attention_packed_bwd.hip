@@ -38,7 +38,7 @@ __device__ __forceinline__ void dq_block(f32x16 (&acc)[DP / 32], const char* kt,
 }
 
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_kernel(const Args p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void packed_attn_dq_kernel(const Args p) {
     typedef Op<T> O;
     constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32, ROW = DP * (int)sizeof(T) + 16;
     constexpr bool EXACT = sizeof(T) == 4;
@@ -187,7 +187,7 @@ __device__ __forceinline__ void dkv_block(f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP
 }
 
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_dkv_kernel(const Args p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void packed_attn_dkv_kernel(const Args p) {
     typedef Op<T> O;
     constexpr int QT = 32, ROW = DP * (int)sizeof(T) + 16;
     constexpr bool VLDS = sizeof(T) == 2;                                               // V's rows stay in LDS, K's in registers

@@ -16,7 +16,7 @@ namespace {
 using namespace pattn;
 
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const Args p) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void packed_attn_fwd_kernel(const Args p) {
     typedef Op<T> O;
     constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32, ROW = DP * (int)sizeof(T) + 16;
     constexpr bool EXACT = sizeof(T) == 4;
