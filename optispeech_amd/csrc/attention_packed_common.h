@@ -55,6 +55,7 @@ template <> struct Op<__bf16> {
     // X as the B operand of a value product: 2 steps of 16 rows
     struct Cols { Frag f[2]; };
     static __device__ __forceinline__ void set(Cols& x, int i, float p) { x.f[i >> 3][i & 7] = (__bf16)p; }   // probabilities enter the matrix pipe as bf16
+    static __device__ __forceinline__ float get(const Cols& x, int i) { return (float)x.f[i >> 3][i & 7]; }
     // Which channels a result block holds: rows 0 .. 15 of block d are the channels 16 d .., rows 16 .. 31 the channels DP / 2 + 16 d .. : the four
     // 16-lane groups of a transposing read then touch different banks (rows are one chunk apart, the two column groups half a row): 2 instead of
     // 8 cycles of LDS a read.
@@ -99,6 +100,7 @@ template <> struct Op<float> {
     static __device__ __forceinline__ f32x16 mma(float a, float b, const f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
     struct Cols { f32x16 f; };
     static __device__ __forceinline__ void set(Cols& x, int i, float p) { x.f[i] = p; }
+    static __device__ __forceinline__ float get(const Cols& x, int i) { return x.f[i]; }
     template <int DP> static __device__ __forceinline__ int channel(int d, int g4, int half) { return 32 * d + g4 * 8 + 4 * half; }
     template <int DP> static __device__ __forceinline__ void value(f32x16 (&y)[DP / 32], const Cols& x, const char* w_l, int lane) {
         constexpr int ROW = DP * 4 + 16;

@@ -15,7 +15,10 @@
 namespace {
 using namespace pattn;
 
-template <typename T, int DP, int MODE>
+// FINE (for a backward, bf16): a probability enters the value product as two bf16 numbers, p = hi + lo.  With one, o is off by 2^-9 of its largest terms, and
+// delta = sum dO O with it: the same amount in every element of a row of dS, which a peaked softmax carries into dQ and dK (error of dQ on 18 k rows with
+// capped scores of deviation 4: 2.8e-3 -> 2.4e-3, what rounding dS and dQ alone gives).
+template <typename T, int DP, int MODE, bool FINE>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void packed_attn_fwd_kernel(const Args p) {
     typedef Op<T> O;
     constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32, ROW = DP * (int)sizeof(T) + 16;
@@ -102,14 +105,16 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void packed_attn_fwd_kernel(
             const float shift = sc.fb - m_run;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                typename O::Cols pc;
+                typename O::Cols pc, lo;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float e = __builtin_amdgcn_exp2f(fmaf(st[b][i], sc.fa, shift));
                     l_run += e;
                     O::set(pc, i, e);
+                    if constexpr (FINE) O::set(lo, i, e - O::get(pc, i));
                 }
                 O::template value<DP>(oacc, pc, vl + b * 32 * ROW, lane);
+                if constexpr (FINE) O::template value<DP>(oacc, lo, vl + b * 32 * ROW, lane);
             }
         }
         if (t + 1 < nt) {
@@ -143,7 +148,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void packed_attn_fwd_kernel(
 // The same for few tiles: a workgroup takes 32 queries of a head and its 4 waves walk the keys in turn, each through its own part of LDS and without
 // barriers, and join their maxima, sums and outputs in LDS at the end.  Four times the workgroups, each a quarter as long, for four times the
 // passes over K and V (out of L2 at these sizes).
-template <typename T, int DP, int MODE>
+template <typename T, int DP, int MODE, bool FINE>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_fwd_split_kernel(const Args p) {
     typedef Op<T> O;
     constexpr int ROW = DP * (int)sizeof(T) + 16, REGION = 2 * 32 * ROW;
@@ -215,15 +220,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_fwd_s
 #pragma unroll
                 for (int i = 0; i < 16; ++i) oacc[d][i] *= alpha;
         }
-        typename O::Cols pc;
+        typename O::Cols pc, lo;
         const float shift = sc.fb - m_run;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float e = __builtin_amdgcn_exp2f(fmaf(st[i], sc.fa, shift));
             l_run += e;
             O::set(pc, i, e);
+            if constexpr (FINE) O::set(lo, i, e - O::get(pc, i));
         }
         O::template value<DP>(oacc, pc, vl, lane);
+        if constexpr (FINE) O::template value<DP>(oacc, lo, vl, lane);
     }
     l_run = half_sum(l_run);
     if (half == 0) { ml[wave][0][l31] = m_run; ml[wave][1][l31] = l_run; }
@@ -263,28 +270,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_fwd_s
     }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool FINE>
 void launch(const Args& p, hipStream_t s) {
     const int mode = (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0);
-    if (split_waves(p.Mq, p.docs, p.Hq, p.klongest, sizeof(T) == 4, false)) {
-        const dim3 grid((unsigned)(p.cap_tiles * p.Hq * 4));
-#define L(M_) hipLaunchKernelGGL((packed_attn_fwd_split_kernel<T, DP, M_>), grid, dim3(256), 0, s, p)
-        if (mode == 0) L(0); else if (mode == 1) L(1); else if (mode == 2) L(2); else L(3);
-#undef L
-        return;
-    }
-    const dim3 grid((unsigned)(p.cap_tiles * p.Hq));
-#define L(M_) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, M_>), grid, dim3(256), 0, s, p)
-    if (mode == 0) L(0); else if (mode == 1) L(1); else if (mode == 2) L(2); else L(3);
+    const bool split = split_waves(p.Mq, p.docs, p.Hq, p.klongest, sizeof(T) == 4, false);
+    const dim3 grid((unsigned)(p.cap_tiles * p.Hq * (split ? 4 : 1)));
+#define L(M_)                                                                                                        \
+    if (split) hipLaunchKernelGGL((packed_attn_fwd_split_kernel<T, DP, M_, FINE>), grid, dim3(256), 0, s, p);        \
+    else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, M_, FINE>), grid, dim3(256), 0, s, p)
+    if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else { L(3); }
 #undef L
 }
-template <typename T>
+template <typename T, bool FINE>
 void launch_width(const Args& p, hipStream_t s) {
     switch (padded_width(p.D)) {
-        case 32: launch<T, 32>(p, s); break;
-        case 64: launch<T, 64>(p, s); break;
-        case 96: launch<T, 96>(p, s); break;
-        default: launch<T, 128>(p, s);
+        case 32: launch<T, 32, FINE>(p, s); break;
+        case 64: launch<T, 64, FINE>(p, s); break;
+        case 96: launch<T, 96, FINE>(p, s); break;
+        default: launch<T, 128, FINE>(p, s);
     }
 }
 }  // namespace
@@ -308,7 +311,9 @@ extern "C" int osp_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_
     p.qlen = qlen; p.kbegin = kbegin; p.klen = klen; p.tiles = reinterpret_cast<const PackedTile*>(qtiles); p.ntiles = qntiles;
     p.prefix = prefix; p.slopes = slopes; p.Mq = Mq; p.docs = docs; p.klongest = klongest; p.cap_tiles = (int)qcap; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk); p.D = (int)D;
     p.causal = (int)(causal != 0); p.scale = scale; p.softcap = softcap;
-    if (bf16) launch_width<__bf16>(p, stream); else launch_width<float>(p, stream);
+    if (!bf16) launch_width<float, false>(p, stream);
+    else if (rest) launch_width<__bf16, true>(p, stream);
+    else launch_width<__bf16, false>(p, stream);
     OSP_LAUNCH_CHECK();
     return OSP_OK;
 }
