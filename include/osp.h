@@ -118,8 +118,11 @@ int osp_attn_softmax_bwd(const float* P, float* dPd, int64_t rows, int64_t T2, f
 int osp_attn_fused_fwd(const float* q, const float* k, const float* v, const int64_t* klen, float* o, int64_t B, int64_t H, int64_t T, int64_t DK, float scale, hipStream_t stream);
 
 /* ---- attention_packed_bwd.hip ---- */
+/* replaces: workspace query for osp_packed_attention_bwd */
+int64_t osp_packed_attention_bwd_workspace_bytes(int64_t docs, int64_t qlongest, int64_t Mk, int64_t Hq, int64_t Hk, int64_t D, int64_t bf16);
+
 /* replaces: autograd of the same: probabilities recomputed per tile from q, k and the log-sum-exp */
-int osp_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* o, const void* rest, const float* lse, const void* dout, int64_t do_row, int64_t do_head, int64_t bf16, void* dq, void* dk, void* dv, float* delta, const int64_t* qbegin, const int64_t* qlen, const int32_t* qtiles, const int32_t* qntiles, int64_t qcap, const int64_t* kbegin, const int64_t* klen, const int32_t* ktiles, const int32_t* kntiles, int64_t kcap, const int64_t* prefix, const float* slopes, int64_t docs, int64_t qlongest, int64_t klongest, int64_t Mq, int64_t Mk, int64_t Hq, int64_t Hk, int64_t D, float scale, float softcap, int64_t causal, hipStream_t stream);
+int osp_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* o, const void* rest, const float* lse, const void* dout, int64_t do_row, int64_t do_head, int64_t bf16, void* dq, void* dk, void* dv, float* delta, void* workspace, const int64_t* qbegin, const int64_t* qlen, const int32_t* qtiles, const int32_t* qntiles, int64_t qcap, const int64_t* kbegin, const int64_t* klen, const int32_t* ktiles, const int32_t* kntiles, int64_t kcap, const int64_t* prefix, const float* slopes, int64_t docs, int64_t qlongest, int64_t klongest, int64_t Mq, int64_t Mk, int64_t Hq, int64_t Hk, int64_t D, float scale, float softcap, int64_t causal, hipStream_t stream);
 
 /* ---- attention_packed_fwd.hip ---- */
 /* replaces: MultiHeadedAttention.forward_attention on packed documents, with capped scores, a penalty on distance, causal and prefix masks, shared key heads and different query / key counts (generator/modules/_transformer/attention.py:75-125 knows a key-padding mask) */

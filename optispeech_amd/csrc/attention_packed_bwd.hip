@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void 
     constexpr bool EXACT = sizeof(T) == 4;
     __shared__ __attribute__((aligned(16))) char lds[2][2][QT * ROW];                  // [buffer][Q, dO]
     __shared__ __attribute__((aligned(16))) float stat[2][2][QT];                      // [buffer][b - log2-sum-exp, -delta]
-    const int hk = blockIdx.x % p.Hk, ti = blockIdx.x / p.Hk;
+    const int hk = blockIdx.x % p.Hk, part = blockIdx.x / p.Hk % p.parts, ti = blockIdx.x / p.Hk / p.parts;
     const int ndoc = p.ntiles[0];
     if (ti >= p.ntiles[1]) return;
     // under a causal mask the first keys have the most queries: the list from its other end
@@ -204,10 +204,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void 
     const int w0 = wave * 32, ki = w0 + l31;
     const int64_t krow = (int64_t)tile.row0 + ki;
     const bool on = ki < tile.n;
-    T* outk = reinterpret_cast<T*>(p.dk) + (krow * p.Hk + hk) * p.D;
-    T* outv = reinterpret_cast<T*>(p.dv) + (krow * p.Hk + hk) * p.D;
+    const int64_t at = (krow * p.Hk + hk) * p.D;
+    T* outk = reinterpret_cast<T*>(p.dk) + at;
+    T* outv = reinterpret_cast<T*>(p.dv) + at;
     if (tile.doc < 0) {
-        if (on)
+        if (on && p.parts == 1)
             for (int d = half * 8; d < p.D; d += 16)
                 for (int e = 0; e < 8; ++e) { outk[d + e] = (T)0.f; outv[d + e] = (T)0.f; }
         return;
@@ -234,13 +235,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void 
 #pragma unroll
         for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
     const int key = tile.i0 + ki;                                                      // this lane's key in the document
-    const int nqt = first < qlen ? (qlen - first + QT - 1) / QT : 0, nt = nqt * p.G;
-    Score<MODE, EXACT> sc(p, hk * p.G);
+    const int nqt = first < qlen ? (qlen - first + QT - 1) / QT : 0, nt = nqt * (p.G / p.parts);
+    const int h0 = hk * p.G + part * (p.G / p.parts);                                  // the first of this workgroup's heads
+    Score<MODE, EXACT> sc(p, h0);
     const float back = p.scale * sc.grad_scale;
     Stage<T, DP, QT, 256> qs(p.qr, p.D, tid), dos(p.dor, p.D, tid);
     float st_reg = 0.f;
     auto load = [&](int t) {
-        const int h = hk * p.G + t / nqt, r0 = first + (t % nqt) * QT;
+        const int h = h0 + t / nqt, r0 = first + (t % nqt) * QT;
         qs.load(reinterpret_cast<const T*>(p.q) + (qb + r0) * p.qr + (int64_t)h * p.qh, p.qr, qlen - r0);
         dos.load(reinterpret_cast<const T*>(p.dout) + (qb + r0) * p.dor + (int64_t)h * p.doh, p.dor, qlen - r0);
         if (tid < 2 * QT) {
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void 
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
         const int buf = t & 1, r0 = first + (t % nqt) * QT;
-        sc.set_head(p, hk * p.G + t / nqt);
+        sc.set_head(p, h0 + t / nqt);
         const char *ql = lds[buf][0], *dl = lds[buf][1];
         const int pos0 = off + r0;
         // the wave's keys are all behind the tile's last query: nothing seen
@@ -284,7 +286,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void 
             const int c = O::template channel<DP>(d, g, half);
             const float a[4] = {dk[d][4 * g] * back, dk[d][4 * g + 1] * back, dk[d][4 * g + 2] * back, dk[d][4 * g + 3] * back};
             const float b[4] = {dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
-            if (c < p.D) { PackedVec<T, 4>::store(outk + c, a); PackedVec<T, 4>::store(outv + c, b); }
+            if (c >= p.D) continue;
+            if (p.parts > 1) {
+                PackedVec<float, 4>::store(p.partial + part * p.part_size + at + c, a);
+                PackedVec<float, 4>::store(p.partial + (p.parts + part) * p.part_size + at + c, b);
+            } else { PackedVec<T, 4>::store(outk + c, a); PackedVec<T, 4>::store(outv + c, b); }
         }
 }
 
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void packe
     __shared__ __attribute__((aligned(16))) char v_l[VLDS ? 32 * ROW : 16];
     __shared__ __attribute__((aligned(16))) char lds[4][REGION];                        // per wave: Q, dO
     __shared__ __attribute__((aligned(16))) float stat[4][2][QT];
-    const int hk = blockIdx.x % p.Hk, ti = blockIdx.x / p.Hk / 4, k0 = (blockIdx.x / p.Hk & 3) * 32;
+    const int hk = blockIdx.x % p.Hk, part = blockIdx.x / p.Hk % p.parts, ti = blockIdx.x / p.Hk / p.parts / 4, k0 = (blockIdx.x / p.Hk / p.parts & 3) * 32;
     const int ndoc = p.ntiles[0];
     if (ti >= p.ntiles[1]) return;
     const PackedTile tile = p.tiles[p.causal && ti < ndoc ? ndoc - 1 - ti : ti];
@@ -413,10 +419,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void packe
     T* outk = reinterpret_cast<T*>(p.dk) + row0 * orow + hk * p.D;
     T* outv = reinterpret_cast<T*>(p.dv) + row0 * orow + hk * p.D;
     if (tile.doc < 0) {
-        zero_head_rows(outk, orow, nk, p.D, tid);
-        zero_head_rows(outv, orow, nk, p.D, tid);
+        if (p.parts == 1) {
+            zero_head_rows(outk, orow, nk, p.D, tid);
+            zero_head_rows(outv, orow, nk, p.D, tid);
+        }
         return;
     }
+    float* partial = p.partial + part * p.part_size + row0 * orow + hk * p.D;
     const int qlen = (int)p.qlen[tile.doc], klen = (int)p.klen[tile.doc];
     const int prefix = p.prefix ? (int)min(max(p.prefix[tile.doc], (int64_t)0), (int64_t)klen) : 0;
     const int64_t qb = p.qbegin[tile.doc];
@@ -436,13 +445,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void packe
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) { dk[d] = splat(0.f); dv[d] = splat(0.f); }
-    const int nqt = first < qlen ? (qlen - first + QT - 1) / QT : 0, nt = nqt * p.G;
-    Score<MODE, EXACT> sc(p, hk * p.G);
+    const int nqt = first < qlen ? (qlen - first + QT - 1) / QT : 0, nt = nqt * (p.G / p.parts);
+    const int h0 = hk * p.G + part * (p.G / p.parts);                                  // the first of this workgroup's heads
+    Score<MODE, EXACT> sc(p, h0);
     Stage<T, DP, QT, 64> qs(p.qr, p.D, lane), dos(p.dor, p.D, lane);
     float st_reg = 0.f;
     char *ql = lds[wave], *dl = lds[wave] + 32 * ROW;
     auto load = [&](int t) {
-        const int h = hk * p.G + t / nqt, r0 = first + (t % nqt) * QT;
+        const int h = h0 + t / nqt, r0 = first + (t % nqt) * QT;
         qs.load(reinterpret_cast<const T*>(p.q) + (qb + r0) * p.qr + (int64_t)h * p.qh, p.qr, qlen - r0);
         dos.load(reinterpret_cast<const T*>(p.dout) + (qb + r0) * p.dor + (int64_t)h * p.doh, p.dor, qlen - r0);
         const float* src = half == 0 ? p.lse : p.delta;
@@ -457,18 +467,51 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void packe
         stat[wave][half][l31] = st_reg;
         __builtin_amdgcn_wave_barrier();
         if (AHEAD && t + 4 < nt) load(t + 4);
-        sc.set_head(p, hk * p.G + t / nqt);
+        sc.set_head(p, h0 + t / nqt);
         const int pos0 = off + first + (t % nqt) * QT;
         dkv_block<T, DP, MODE>(dk, dv, ql, dl, stat[wave][0], stat[wave][1], kf, vf, v_l, sc, pos0, key, prefix, p.causal && pos0 < i0 + 31, lane);
     }
     __builtin_amdgcn_wave_barrier();
     put_rows<DP>(reinterpret_cast<float*>(lds[wave]), dk, p.scale * sc.grad_scale, l31, half, &O::template channel<DP>);
     __syncthreads();
-    add_rows<T, DP, REGION>(outk, orow, lds, nk, p.D, tid);
+    if (p.parts > 1) add_rows<float, DP, REGION>(partial, orow, lds, nk, p.D, tid);
+    else add_rows<T, DP, REGION>(outk, orow, lds, nk, p.D, tid);
     __syncthreads();
     put_rows<DP>(reinterpret_cast<float*>(lds[wave]), dv, 1.f, l31, half, &O::template channel<DP>);
     __syncthreads();
-    add_rows<T, DP, REGION>(outv, orow, lds, nk, p.D, tid);
+    if (p.parts > 1) add_rows<float, DP, REGION>(partial + p.parts * p.part_size, orow, lds, nk, p.D, tid);
+    else add_rows<T, DP, REGION>(outv, orow, lds, nk, p.D, tid);
+}
+
+// dK and dV from the parts of their heads, in the order of the parts; rows of no document become zeros
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_parts_kernel(const Args p) {
+    const PackedTile tile = p.tiles[blockIdx.x];
+    if ((int)blockIdx.x >= p.ntiles[1]) return;
+    const int64_t row = (int64_t)p.Hk * p.D, first = tile.row0 * row;
+    const int quads = (int)(tile.n * row / 4);
+    T* out = reinterpret_cast<T*>(blockIdx.y ? p.dv : p.dk);
+    const float* in = p.partial + blockIdx.y * p.parts * p.part_size;
+    for (int u = blockIdx.z * 256 + threadIdx.x; u < quads; u += 256 * gridDim.z) {
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        if (tile.doc >= 0)
+            for (int i = 0; i < p.parts; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(in + i * p.part_size + first + 4 * (int64_t)u);
+                a[0] += v.x; a[1] += v.y; a[2] += v.z; a[3] += v.w;
+            }
+        PackedVec<T, 4>::store(out + first + 4 * (int64_t)u, a);
+    }
+}
+
+// dK / dV: waves that share 32 keys, and parts the query heads of a key head are cut into, where the workgroups would not fill the chip evenly (one part:
+// the sum over the heads stays in registers).  16 heads sharing 4, causal documents of up to 8192 rows, 568 tiles of up to 1024 steps: 2.83 ms in one part,
+// 2.46 ms and 0.11 ms for the sums in four.  The waves that share 32 keys are four times as many workgroups already: parts only below one a CU.
+struct KeyPlan { bool split; int parts; };
+KeyPlan plan_keys(int64_t rows, int64_t docs, int64_t Hk, int64_t G, int64_t qlongest, int64_t D, bool f32) {
+    KeyPlan r = {split_waves(rows, docs, Hk, qlongest * G, f32, padded_width(D) > 64), 1};
+    const int64_t n = (rows / PACKED_TILE + docs / 2) * Hk * (r.split ? 4 : 1), want = r.split ? 256 : 2048;
+    while (r.parts < G && n * r.parts < want) { do ++r.parts; while (G % r.parts); }
+    return r;
 }
 
 template <typename T, int DP>
@@ -476,8 +519,8 @@ void launch(Args p, const PackedTile* ktiles, const int* kntiles, int kcap, hipS
     const int mode = (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0);
     Args pk = p;
     pk.tiles = ktiles; pk.ntiles = kntiles; pk.cap_tiles = kcap;
-    const bool sq = split_waves(p.Mq, p.docs, p.Hq, p.klongest, sizeof(T) == 4, DP > 64), sk = split_waves(p.Mk, p.docs, p.Hk, p.qlongest * p.G, sizeof(T) == 4, DP > 64);
-    const dim3 gq((unsigned)(p.cap_tiles * p.Hq * (sq ? 4 : 1))), gk((unsigned)(kcap * p.Hk * (sk ? 4 : 1)));
+    const bool sq = split_waves(p.Mq, p.docs, p.Hq, p.klongest, sizeof(T) == 4, DP > 64), sk = plan_keys(p.Mk, p.docs, p.Hk, p.G, p.qlongest, p.D, sizeof(T) == 4).split;
+    const dim3 gq((unsigned)(p.cap_tiles * p.Hq * (sq ? 4 : 1))), gk((unsigned)(kcap * p.Hk * p.parts * (sk ? 4 : 1)));
 #define L(M_)                                                                                       \
     if (sq) hipLaunchKernelGGL((packed_attn_dq_split_kernel<T, DP, M_>), gq, dim3(256), 0, s, p);    \
     else hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, M_>), gq, dim3(256), 0, s, p);             \
@@ -485,6 +528,7 @@ void launch(Args p, const PackedTile* ktiles, const int* kntiles, int kcap, hipS
     else hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, M_>), gk, dim3(256), 0, s, pk)
     if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else { L(3); }
 #undef L
+    if (p.parts > 1) hipLaunchKernelGGL((packed_attn_parts_kernel<T>), dim3((unsigned)kcap, 2, 4), dim3(256), 0, s, pk);
 }
 template <typename T>
 void launch_width(const Args& p, const PackedTile* kt, const int* kn, int kcap, hipStream_t s) {
@@ -497,9 +541,16 @@ void launch_width(const Args& p, const PackedTile* kt, const int* kn, int kcap, 
 }
 }  // namespace
 
+// Bytes of the workspace of the backward (0: none needed).
+extern "C" int64_t osp_packed_attention_bwd_workspace_bytes(int64_t docs, int64_t qlongest, int64_t Mk, int64_t Hq, int64_t Hk, int64_t D, int64_t bf16) {
+    if (docs <= 0 || Mk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0) return 0;
+    const int64_t parts = plan_keys(Mk, docs, Hk, Hq / Hk, qlongest, D, !bf16).parts;
+    return parts > 1 ? 2 * parts * Mk * Hk * D * 4 : 0;
+}
+
 extern "C" int osp_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
                                         int64_t v_row, int64_t v_head, const void* o, const void* rest, const float* lse, const void* dout, int64_t do_row,
-                                        int64_t do_head, int64_t bf16, void* dq, void* dk, void* dv, float* delta, const int64_t* qbegin,
+                                        int64_t do_head, int64_t bf16, void* dq, void* dk, void* dv, float* delta, void* workspace, const int64_t* qbegin,
                                         const int64_t* qlen, const int32_t* qtiles, const int32_t* qntiles, int64_t qcap, const int64_t* kbegin,
                                         const int64_t* klen, const int32_t* ktiles, const int32_t* kntiles, int64_t kcap, const int64_t* prefix,
                                         const float* slopes, int64_t docs, int64_t qlongest, int64_t klongest, int64_t Mq, int64_t Mk,
@@ -522,6 +573,11 @@ extern "C" int osp_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_
     p.qbegin = qbegin; p.qlen = qlen; p.kbegin = kbegin; p.klen = klen; p.tiles = reinterpret_cast<const PackedTile*>(qtiles); p.ntiles = qntiles;
     p.prefix = prefix; p.slopes = slopes; p.Mq = Mq; p.Mk = Mk; p.docs = docs; p.qlongest = qlongest; p.klongest = klongest; p.cap_tiles = (int)qcap; p.Hq = (int)Hq; p.Hk = (int)Hk; p.G = (int)(Hq / Hk); p.D = (int)D;
     p.causal = (int)(causal != 0); p.scale = scale; p.softcap = softcap;
+    p.parts = plan_keys(Mk, docs, Hk, Hq / Hk, qlongest, D, !bf16).parts;
+    p.part_size = Mk * Hk * D;
+    p.partial = reinterpret_cast<float*>(workspace);
+    OSP_CHECK_ARG(p.parts == 1 || (workspace && packed_aligned(workspace, 16)), "workspace missing: osp_packed_attention_bwd_workspace_bytes");
+    OSP_CHECK_ARG(kcap * Hk * p.parts < (int64_t)1 << 29, "too many tiles");
     const PackedTile* kt = reinterpret_cast<const PackedTile*>(ktiles);
     if (bf16) launch_width<__bf16>(p, kt, kntiles, (int)kcap, stream); else launch_width<float>(p, kt, kntiles, (int)kcap, stream);
     OSP_LAUNCH_CHECK();

@@ -41,7 +41,9 @@ struct Args {
     const int64_t* prefix;                              // per document or null
     const float* slopes;                                // per query head or null
     int64_t Mq, Mk, docs, qlongest, klongest;           // the last two: the host's bounds on a document, used to choose a kernel only
-    int cap_tiles, Hq, Hk, G, D, causal;
+    float* partial;                                     // dK, dV of the parts of a key head's query heads: (2, parts, Mk, Hk, D)
+    int64_t part_size;
+    int cap_tiles, Hq, Hk, G, D, causal, parts;
     float scale, softcap;
 };
 

@@ -15,6 +15,7 @@ import math
 
 import torch
 
+from . import _lib
 from . import precision as _precision
 from ._lib import OspError, call, lib
 from .ops import _want
@@ -35,6 +36,11 @@ def _wants_grad(*ts):
     return torch.is_grad_enabled() and not torch.is_inference_mode_enabled() and any(t.requires_grad for t in ts)
 
 
+def _first_order():
+    if torch.is_grad_enabled():                                   # create_graph: the gradients below would enter the graph as constants
+        raise OspError("the packed operators have no second derivatives (create_graph=True)")
+
+
 class PackedRows:
     """Documents of a table of ``rows`` rows: ``begin`` / ``length`` (docs,) int64 on the device, the tile list of the kernels, and the
     host's upper bound ``longest`` on a document's length."""
@@ -49,7 +55,9 @@ class PackedRows:
         self.docs, self.rows, self.longest, self.device = docs, rows, min(longest, rows), src.device
         self.cap = _size("osp_packed_rows_tiles", docs, rows)
         long = torch.empty((2, docs), device=src.device, dtype=torch.int64)
+        self._buffers, self._stream = [long], _lib._raw_stream(src.device.index)
         ints = torch.empty((4 * self.cap + docs + 2,), device=src.device, dtype=torch.int32)
+        self._buffers.append(ints)
         self.begin, self.length = long[0], long[1]
         self.tiles, self.base, self.ntiles = ints[:4 * self.cap], ints[4 * self.cap:4 * self.cap + docs], ints[4 * self.cap + docs:]
         call("osp_packed_rows_plan", src, int(padded), docs, rows, rows // docs if padded else 0, self.begin, self.length, self.base, self.tiles,
@@ -72,6 +80,10 @@ class PackedRows:
             raise OspError(f"{name} has {t.shape[0]} rows, the documents were laid out for {self.rows}")
         if t.device != self.device:
             raise OspError(f"{name} is on {t.device}, the documents on {self.device}")
+        if _lib._raw_stream(self.device.index) != self._stream:
+            # used on another stream than it was built on (the caller orders the two): its memory must outlive that stream's work
+            for b in self._buffers:
+                b.record_stream(torch.cuda.current_stream(self.device))
 
 
 # ------------------------------------------------------------------------------------------------------------------ rotary positions
@@ -146,6 +158,7 @@ class RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
+        _first_order()
         rope, rows, first, dtype = ctx.cfg
         qs, ks, od, dev = ctx.shapes
         dq = torch.zeros(qs, device=dev, dtype=od) if dq is None else dq.to(od)
@@ -228,6 +241,7 @@ class GroupNormFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _first_order()
         x, stats = ctx.saved_tensors
         (w, b), (groups, rows, act) = ctx.params, ctx.cfg
         M, C = x.shape
@@ -284,7 +298,9 @@ def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):
     o = torch.empty((M, H, D), device=q.device, dtype=q.dtype)
     lse = torch.empty((H, M), device=q.device, dtype=torch.float32) if save else None
     rest = torch.empty_like(o) if save and bf16 else None
-    if M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536:
+    if not k.shape[0]:                                            # no keys at all: nothing is seen
+        o.zero_()
+    elif M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536:
         # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip)
         ws = _workspace(_size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D), q.device)
         call("osp_packed_attention_token", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, ws,
@@ -307,6 +323,7 @@ class PackedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do):
+        _first_order()
         q, k, v, o, rest, lse, prefix, slopes = ctx.saved_tensors
         rows, keys, causal, softcap, scale = ctx.cfg
         (M, H, D), (Mk, S, _) = q.shape, k.shape
@@ -315,8 +332,10 @@ class PackedAttentionFn(torch.autograd.Function):
         dk, dv = (torch.empty((Mk, S, D), device=q.device, dtype=q.dtype) for _ in range(2))
         if M and Mk:
             delta = torch.empty_like(lse)
+            nbytes = _size("osp_packed_attention_bwd_workspace_bytes", rows.docs, rows.longest, Mk, H, S, D, int(q.dtype == torch.bfloat16))
+            ws = _workspace(nbytes, q.device) if nbytes else None
             call("osp_packed_attention_bwd", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), o, rest, lse, do,
-                 do.stride(0), do.stride(1), int(q.dtype == torch.bfloat16), dq, dk, dv, delta, rows.begin, rows.length, rows.tiles, rows.ntiles,
+                 do.stride(0), do.stride(1), int(q.dtype == torch.bfloat16), dq, dk, dv, delta, ws, rows.begin, rows.length, rows.tiles, rows.ntiles,
                  rows.cap, keys.begin, keys.length, keys.tiles, keys.ntiles, keys.cap, prefix, slopes, rows.docs, rows.longest, keys.longest, M, Mk, H, S, D,
                  scale, softcap, causal)
         else:

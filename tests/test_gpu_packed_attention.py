@@ -117,6 +117,47 @@ def test_attention_forward_and_gradients(dtype, mask, cap, slope, lengths, tail,
     close(got, want, tol)
 
 
+MANY = [5, 0, 33, 127, 128, 129, 1, 64, 31, 65] * 6
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask,cap,slope", [("full", 0.0, False), ("full", 0.0, True), ("causal", 5.0, False), ("prefix", 20.0, True), ("causal", 0.0, True)])
+@pytest.mark.parametrize("H,S,D", [(8, 8, 128), (8, 4, 64), (10, 5, 40), (16, 4, 96), (12, 4, 32)])
+def test_attention_over_many_documents(dtype, mask, cap, slope, H, S, D):
+    """enough tiles for the kernels whose waves own 32 rows each, and for key heads whose query heads are cut into parts; forward and gradients"""
+    from optispeech_amd import packed_ops as P
+    M = sum(MANY) + 6
+    q, do = randn(M, H, D, seed=1, dtype=dtype, std=3.0 if cap else 1.0), randn(M, H, D, seed=4, dtype=dtype)
+    k, v = randn(M, S, D, seed=2, dtype=dtype), randn(M, S, D, seed=3, dtype=dtype)
+    prefix = torch.tensor([(7 * i + 3) % (n + 2) for i, n in enumerate(MANY)], dtype=torch.int64, device=DEV) if mask == "prefix" else None
+    slopes = torch.tensor([0.5 ** (h + 1) for h in range(H)], device=DEV) if slope else None
+    rows = P.PackedRows.from_offsets(offsets(MANY), M, longest=max(MANY))
+    got = grads(q, k, v, do, rows, causal=mask != "full", prefix=prefix, softcap=cap, slopes=slopes)
+    docs = ref.documents(MANY)
+    want, tol = bounds(q, k, v, do, docs, docs, D ** -0.5, mask != "full", prefix, cap, slopes, dtype)
+    close(got, want, tol)
+    for t in got:
+        assert float(t.detach()[sum(MANY):].abs().sum()) == 0.0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_documents(dtype):
+    """documents of many tiles, queries and keys of different numbers, in both arrangements of the waves"""
+    from optispeech_amd import packed_ops as P
+    for qlens, klens, H, S, D in (([1500, 700], [1500, 900], 2, 1, 64), ([900] * 6, [1100, 900, 130, 900, 901, 1000], 12, 6, 128)):
+        M, Mk = sum(qlens), sum(klens)
+        q, do = randn(M, H, D, seed=1, dtype=dtype), randn(M, H, D, seed=4, dtype=dtype)
+        k, v = randn(Mk, S, D, seed=2, dtype=dtype), randn(Mk, S, D, seed=3, dtype=dtype)
+        prefix = torch.tensor([300 * i for i in range(len(qlens))], dtype=torch.int64, device=DEV)
+        rows = P.PackedRows.from_offsets(offsets(qlens), M, longest=max(qlens))
+        keys = P.PackedRows.from_offsets(offsets(klens), Mk, longest=max(klens))
+        got = grads(q, k, v, do, rows, keys=keys, causal=True, prefix=prefix)
+        want, tol = bounds(q, k, v, do, ref.documents(qlens), ref.documents(klens), D ** -0.5, True, prefix, 0.0, None, dtype)
+        close(got, want, tol)
+
+
 @gpu
 def test_the_bounds_reference_agrees_with_autograd():
     """the gradient formulas above against autograd of the plain definition (float64, CPU)"""
@@ -319,6 +360,94 @@ def test_captured_forward_replayed_with_other_lengths():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, step()), lens
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_training_step_replayed(dtype):
+    """rows, rotary, attention, group norm and their backward in one graph; every replay, with eager work in between, equals the eager step bit for bit"""
+    from optispeech_amd import packed_ops as P
+    M, H, S, D = 260, 4, 2, 32
+    off = offsets([100, 130])
+    x, g = randn(M, (H + 2 * S) * D, seed=1, dtype=dtype).requires_grad_(), randn(M, H * D, seed=5, dtype=dtype)
+    w, b = torch.nn.Parameter(randn(H * D, seed=2)), torch.nn.Parameter(randn(H * D, seed=3))
+    w.grad, b.grad = torch.zeros_like(w), torch.zeros_like(b)
+    rope = P.Rotary(D, layout="interleaved")
+
+    def step():
+        w.grad.zero_(), b.grad.zero_()
+        rows = P.PackedRows.from_offsets(off, M)
+        q, k, v = (t.unflatten(1, (-1, D)) for t in x.split([H * D, S * D, S * D], 1))
+        q, k = P.rotary(q, k, rope, rows)
+        o = P.attention(q, k, v, rows, causal=True, softcap=9.0)
+        y = P.group_norm(o.flatten(1), w, b, 4, rows, 1e-5, "gelu")
+        return (y.detach(),) + torch.autograd.grad(y, (x,), g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i, lens in enumerate(([100, 130], [260, 0], [1, 259], [5, 6])):
+        off.copy_(offsets(lens))
+        with torch.no_grad():
+            x.copy_(randn(M, (H + 2 * S) * D, seed=10 + i, dtype=dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out] + [w.grad.clone(), b.grad.clone()]
+        want = list(step()) + [w.grad, b.grad]
+        for a, e in zip(got, want):
+            assert torch.equal(a, e), lens
+
+
+@gpu
+def test_rows_built_on_one_stream_and_used_on_another():
+    """the handle is dropped while the other stream still works: its memory is not handed out before that work is done"""
+    from optispeech_amd import packed_ops as P
+    lengths, H, D = [400, 300], 4, 64
+    M = sum(lengths)
+    q, k, v = (randn(M, H, D, seed=i, dtype=torch.bfloat16) for i in range(3))
+    want = P.attention(q, k, v, P.PackedRows.from_offsets(offsets(lengths), M), causal=True)
+    side = torch.cuda.Stream()
+    outs = []
+    for _ in range(5):
+        rows = P.PackedRows.from_offsets(offsets(lengths), M)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            outs.append(P.attention(q, k, v, rows, causal=True))
+        del rows
+        torch.full((4096,), -1, dtype=torch.int32, device=DEV)      # would take the freed blocks
+    torch.cuda.current_stream().wait_stream(side)
+    for o in outs:
+        assert torch.equal(o, want)
+
+
+@gpu
+def test_empty_tables_and_second_derivatives():
+    """no rows, no keys: zeros of the right shapes; a second derivative is refused, not taken as zero"""
+    from optispeech_amd import packed_ops as P
+    none = P.PackedRows.from_offsets(offsets([0, 0]), 0)
+    some = P.PackedRows.from_offsets(offsets([2, 3]), 5)
+    q0, q5 = torch.zeros(0, 2, 8, device=DEV), randn(5, 2, 8, seed=1)
+    o, dq, dk, dv = grads(q0, q0, q0, q0, none)
+    assert o.shape == dq.shape == dk.shape == dv.shape == (0, 2, 8)
+    o, dq, dk, dv = grads(q5, q0, q0, q5, some, keys=none, causal=True)
+    assert float(o.detach().abs().sum()) == 0.0 and float(dq.abs().sum()) == 0.0 and dk.shape == (0, 2, 8)
+    o, dq, dk, dv = grads(q0, q5, q5, q0, none, keys=some)
+    assert float(dk.abs().sum()) == 0.0 and float(dv.abs().sum()) == 0.0
+    with torch.no_grad():
+        assert float(P.attention(q5, q0, q0, some, keys=none).abs().sum()) == 0.0
+    yq, yk = P.rotary(q0, q0, P.Rotary(8), none)
+    assert yq.shape == (0, 2, 8)
+    assert P.group_norm(q0.flatten(1), torch.ones(16, device=DEV), torch.ones(16, device=DEV), 2, none).shape == (0, 16)
+    q = q5.clone().requires_grad_()
+    w = torch.nn.Parameter(torch.ones(16, device=DEV))
+    from optispeech_amd._lib import OspError
+    for y in (P.attention(q, q, q, some), P.rotary(q, q, P.Rotary(8), some)[0], P.group_norm(q.flatten(1), w, w, 2, some)):
+        with pytest.raises(OspError, match="second"):
+            torch.autograd.grad(y.sum(), (q,), create_graph=True)
 
 
 @gpu

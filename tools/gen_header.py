@@ -148,6 +148,7 @@ REPLACES = {
     "osp_packed_attention_fwd": "MultiHeadedAttention.forward_attention on packed documents, with capped scores, a penalty on distance, causal and prefix "
                                 "masks, shared key heads and different query / key counts (generator/modules/_transformer/attention.py:75-125 "
                                 "knows a key-padding mask)",
+    "osp_packed_attention_bwd_workspace_bytes": "workspace query for osp_packed_attention_bwd",
     "osp_packed_attention_bwd": "autograd of the same: probabilities recomputed per tile from q, k and the log-sum-exp",
     "osp_packed_attention_token_workspace_bytes": "workspace query for osp_packed_attention_token",
     "osp_packed_attention_token": "osp_packed_attention_fwd for few queries over many keys (new frames over a cache): keys split over workgroups and joined",
