@@ -60,7 +60,7 @@ template <> struct Op<__bf16> {
     static __device__ __forceinline__ float get(const Cols& x, int i) { return (float)x.f[i >> 3][i & 7]; }
     // Which channels a result block holds: rows 0 .. 15 of block d are the channels 16 d .., rows 16 .. 31 the channels DP / 2 + 16 d .. : the four
     // 16-lane groups of a transposing read then touch different banks (rows are one chunk apart, the two column groups half a row): 2 instead of
-    // 8 cycles of LDS a read.
+    // 6 conflict cycles a read.
     template <int DP> static __device__ __forceinline__ int channel(int d, int g4, int half) { return 16 * d + (g4 >> 1) * (DP / 2) + (g4 & 1) * 8 + 4 * half; }
     template <int DP> static __device__ __forceinline__ void value(f32x16 (&y)[DP / 32], const Cols& x, const char* w_l, int lane) {
         constexpr int ROW = DP * 2 + 16;

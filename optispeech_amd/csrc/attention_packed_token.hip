@@ -6,6 +6,9 @@
 // its own tiles of 32 keys through its own part of LDS, without barriers: rows are requested into registers one tile ahead (16 KB per wave
 // in flight), stored to LDS, and read back as matrix operands.  The waves' results meet in LDS at the end, the splits' (maximum, sum, unscaled
 // output) go to a workspace in f32, and a second launch joins them in the order of the splits.
+//
+// Measured (bf16): 48 requests of 1 .. 16384 keys, 16 heads of 128 sharing 2: 457 MB in 95.5 us (4.8 TB/s; a copy reaches 5.1) and 6 us for the join;  8 streams
+// of up to 800 keys, 2 heads: 7.8 + 3.9 us, latency.
 #include "attention_packed_common.h"
 
 namespace {

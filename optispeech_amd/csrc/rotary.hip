@@ -8,7 +8,11 @@
 // pi / 4 whose rounding is 2^-25 of it.  sin and cos of it are Taylor sums (degree 9 and 10; the first term left out is below 2e-9).
 //
 // Bound: HBM.  The 64-bit work is done once per row and pair, into LDS, and serves all heads of q and k; the heads are then walked in the order of memory
-// with accesses of 16 bytes where alignment allows.
+// with accesses of 16 bytes where alignment allows.  (A thread that kept its pairs' cos and sin in registers and walked the heads itself read every row
+// in strides of a head: 87 us where this takes 75.)
+//
+// Measured: 24 k rows, 16 + 4 heads of 128, bf16: 75 us, 4.4 TB/s (a copy reaches 5.1);  17 k rows, 4 + 4 heads of 64, half of each turned, f32: 15.1 us, 4.8 TB/s;
+// 8 rows: 4.7 us, latency.
 #include "packed_common.h"
 
 namespace {
