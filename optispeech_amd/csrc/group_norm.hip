@@ -644,6 +644,7 @@ bool try_resident(const NormArgs& p, int act, int64_t longest, bool backward, hi
     else {
         Slab sl;
         if (!packed_aligned(p.w, 16) || !packed_aligned(p.b, 16)) return false;
+        if ((int64_t)p.B * p.G > (int64_t)1 << 21) return false;             // (a launch has fewer than 2^32 threads)
         int nr = plan_slab(longest, p.C, p.G, V, 512, sl);
         if (nr == 0) {
             nr = plan_slab(longest, p.C, p.G, V, 1024, sl);

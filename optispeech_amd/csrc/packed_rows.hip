@@ -124,7 +124,8 @@ extern "C" int64_t osp_packed_rows_tiles(int64_t B, int64_t M) {
 extern "C" int osp_packed_rows_plan(const int64_t* src, int64_t padded, int64_t B, int64_t M, int64_t T, int64_t* begin, int64_t* len,
                                     int32_t* base, int32_t* tiles, int32_t* ntiles, int64_t cap, hipStream_t stream) {
     OSP_CHECK_ARG(src && begin && len && base && tiles && ntiles && B > 0 && M >= 0, "bad args");
-    OSP_CHECK_ARG(M < (int64_t)1 << 31 && B < (int64_t)1 << 24, "at most 2^31 - 1 rows and 2^24 documents");
+    // (row numbers are 32-bit in the kernels, which look up to a few tiles beyond a row)
+    OSP_CHECK_ARG(M <= ((int64_t)1 << 31) - 65536 && B < (int64_t)1 << 24, "at most 2^31 - 65536 rows and 2^24 - 1 documents");
     OSP_CHECK_ARG(!padded || (T >= 0 && T * B == M), "a padded batch has B * T rows");
     OSP_CHECK_ARG(cap >= osp_packed_rows_tiles(B, M), "tile list shorter than osp_packed_rows_tiles(B, M)");
     OSP_CHECK_ARG(packed_aligned(tiles, 16), "tile list must be 16-byte aligned");

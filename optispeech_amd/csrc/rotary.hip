@@ -143,6 +143,7 @@ extern "C" int osp_rotary(const void* q, int64_t q_row, int64_t q_head, const vo
     OSP_CHECK_ARG(q && k && qo && ko && turns && tiles && ntiles, "null pointer");
     OSP_CHECK_ARG(cap > 0 && cap < (int64_t)1 << 31 && Hq > 0 && Hk > 0 && Hq <= 65536 && Hk <= 65536, "bad tile list or head counts");
     OSP_CHECK_ARG(D > 0 && D <= 8192 && R >= 2 && R <= D && R % 2 == 0, "an even number of turned channels, at most the head's");
+    OSP_CHECK_ARG(Hq * D <= 1 << 26 && Hk * D <= 1 << 26, "a row has at most 2^26 channels");
     RotaryArgs p;
     p.x[0] = q; p.x[1] = k; p.y[0] = qo; p.y[1] = ko;
     p.xr[0] = q_row; p.xr[1] = k_row; p.xh[0] = q_head; p.xh[1] = k_head;

@@ -8,6 +8,9 @@ they hold on the way in.
 The handle is built once per batch from device offsets or lengths (no copy to the host) and used by every layer and direction.
 Like the rest of the package: kernels go to torch's current stream on the current device, parameter gradients are accumulated into
 ``param.grad`` by the kernels, activations flow through autograd.
+
+A captured graph reads the handle's tensors at every replay: build the handle inside the capture, or keep it as long as the graph.  As for any
+torch operator, a backward pass is captured while no eager graph of the same leaf activations is alive.
 """
 import ctypes
 import functools
@@ -233,10 +236,11 @@ def _grad_target(p):
 
 class GroupNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, b, groups, rows, eps, act):
+    def forward(ctx, x, anchor, params, groups, rows, eps, act):
+        w, b = params
         x, y, stats = _normalise(x, w, b, groups, rows, eps, act)
         ctx.save_for_backward(x, stats)
-        ctx.params, ctx.cfg = (w, b), (groups, rows, act)
+        ctx.params, ctx.cfg = params, (groups, rows, act)
         return y
 
     @staticmethod
@@ -247,7 +251,8 @@ class GroupNormFn(torch.autograd.Function):
         M, C = x.shape
         dy = _matrix(dy, "dy")
         dx = torch.empty((M, C), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
-        (dw, add_w), (db, add_b) = _grad_target(w), _grad_target(b)
+        db, add_b = _grad_target(b)                                # the kernels write db first, then dw: one tensor may be both
+        dw, add_w = _grad_target(w)
         if M and rows.longest:
             ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 1), x.device)
             call("osp_group_norm_bwd", dy, dy.stride(0), x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, stats, dx, dw, add_w, db, add_b, ws,
@@ -279,7 +284,10 @@ def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
     rows._check(x, "x")
     if not _wants_grad(x, weight, bias):
         return _normalise(x, weight, bias, int(groups), rows, float(eps), ACTS[act])[1]
-    return GroupNormFn.apply(x, weight, bias, int(groups), rows, float(eps), ACTS[act])
+    # The parameters stay out of the autograd graph (the kernels write their gradients), so a captured backward meets no node of an eager graph;
+    # where x has no gradient a leaf of the call's own keeps the backward reachable.
+    anchor = None if x.requires_grad else x.new_empty(0, dtype=torch.float32).requires_grad_()
+    return GroupNormFn.apply(x, anchor, (weight, bias), int(groups), rows, float(eps), ACTS[act])
 
 
 # ------------------------------------------------------------------------------------------------------------------ attention over documents
@@ -298,11 +306,14 @@ def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):
     o = torch.empty((M, H, D), device=q.device, dtype=q.dtype)
     lse = torch.empty((H, M), device=q.device, dtype=torch.float32) if save else None
     rest = torch.empty_like(o) if save and bf16 else None
+    # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip).  Its workspace
+    # holds every row of the table per split, at most 34 MB where the rows are the documents'; a far larger table takes the other form.
+    few = M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536
+    nbytes = _size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D) if few else 0
     if not k.shape[0]:                                            # no keys at all: nothing is seen
         o.zero_()
-    elif M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536:
-        # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip)
-        ws = _workspace(_size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D), q.device)
+    elif few and nbytes <= 1 << 28:
+        ws = _workspace(nbytes, q.device)
         call("osp_packed_attention_token", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, ws,
              rows.begin, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, keys.longest, prefix, slopes, rows.docs, M, H, S,
              D, scale, softcap, causal)

@@ -425,6 +425,71 @@ def test_rows_built_on_one_stream_and_used_on_another():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_broadcast_heads_and_rows(dtype):
+    """one key head expanded over the query heads, one row expanded over the table: results of the contiguous tensors, bit for bit, and the gradient
+    summed over the copies"""
+    from optispeech_amd import packed_ops as P
+    lengths, H, D = [50, 33], 4, 32
+    M = sum(lengths)
+    rows = P.PackedRows.from_offsets(offsets(lengths), M)
+    q, v, do = randn(M, H, D, seed=1, dtype=dtype), randn(M, H, D, seed=3, dtype=dtype), randn(M, H, D, seed=4, dtype=dtype)
+    for shape in ((M, 1, D), (1, H, D), (1, 1, D)):
+        k = randn(*shape, seed=2, dtype=dtype)
+        a, b = k.clone().requires_grad_(), k.clone().requires_grad_()
+        oa, ob = P.attention(q, a.expand(M, H, D), v, rows, causal=True), P.attention(q, b.expand(M, H, D).contiguous(), v, rows, causal=True)
+        assert torch.equal(oa, ob)
+        assert torch.equal(torch.autograd.grad(oa, (a,), do)[0], torch.autograd.grad(ob, (b,), do)[0])
+        with torch.no_grad():
+            assert torch.equal(P.attention(a.expand(M, H, D), v, v, rows), P.attention(a.expand(M, H, D).contiguous(), v, v, rows))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_streams_share_a_handle(dtype):
+    """training and token calls issued on two streams at once, nothing shared but the handles and the inputs"""
+    from optispeech_amd import packed_ops as P
+    lengths, H, D = [200, 133, 1], 4, 64
+    M = sum(lengths)
+    rows = P.PackedRows.from_offsets(offsets(lengths), M)
+    tokens = P.PackedRows.from_offsets(offsets([1, 1, 1]), 3, longest=1)
+    sets = [[randn(M, H, D, seed=10 * j + i, dtype=dtype) for i in range(4)] for j in range(2)]
+    run = lambda t: list(grads(*t, rows, causal=True)) + [P.attention(t[0][:3], t[1], t[2], tokens, keys=rows, causal=True)]      # noqa: E731
+    want = [run(t) for t in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(run(sets[j]))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for result in got[j]:
+            for a, e in zip(result, want[j]):
+                assert torch.equal(a, e)
+
+
+@gpu
+def test_new_tokens_in_a_large_table():
+    """three tokens in a table of a million rows: right, zeros behind them, and no workspace that grows with rows times splits"""
+    from optispeech_amd import packed_ops as P
+    M, H, D, klens = 1000000, 2, 8, [9000, 1, 4000]
+    q = randn(M, H, D, seed=1, dtype=torch.bfloat16)
+    k, v = (randn(sum(klens), H, D, seed=i, dtype=torch.bfloat16) for i in (2, 3))
+    rows = P.PackedRows.from_offsets(offsets([1, 1, 1]), M, longest=1)
+    keys = P.PackedRows.from_offsets(offsets(klens), sum(klens))
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    o = P.attention(q, k, v, rows, keys=keys, causal=True)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 29
+    want, tol = bounds(q[:3], k, v, q[:3], ref.documents([1, 1, 1]), ref.documents(klens), D ** -0.5, True, None, 0.0, None, torch.bfloat16)
+    close((o[:3],), want[:1], tol[:1])
+    assert float(o[3:].abs().max()) == 0.0
+
+
+@gpu
 def test_empty_tables_and_second_derivatives():
     """no rows, no keys: zeros of the right shapes; a second derivative is refused, not taken as zero"""
     from optispeech_amd import packed_ops as P

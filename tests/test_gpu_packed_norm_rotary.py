@@ -151,7 +151,7 @@ def test_rotary_scalings():
 
 # ------------------------------------------------------------------------------------------------------------------ group norm
 CASES = [([1], 0, 8, 2), ([37, 17], 0, 64, 4), ([5, 0, 131, 64], 7, 100, 4), ([700, 3, 129], 1, 384, 8), ([1, 1, 2], 3, 10, 5), ([513], 0, 2048, 32),
-         ([260, 255], 9, 36, 1), ([64], 0, 40, 40)]
+         ([260, 255], 9, 36, 1), ([64], 0, 40, 40), ([800, 5, 450], 2, 128, 2), ([400, 130], 0, 256, 2), ([1100], 0, 32, 2)]
 
 
 @gpu
@@ -305,6 +305,100 @@ def test_group_norm_strided_input_padded_rows_with_nan_and_frozen_weights():
     scale = 40 * U
     assert ((y.detach().double().cpu() - want.detach()).abs() <= scale * (1 + want.detach().abs())).all()
     assert ((dx[:, 1:1 + C].double().cpu() - wx).abs() <= 200 * U * wx.abs().max()).all()
+
+
+@gpu
+def test_group_norm_weights_alone_want_a_gradient():
+    """x without a gradient (the first layer, or a frozen one below): the weights' gradients are those of the full backward"""
+    from optispeech_amd import packed_ops as P
+    for lengths, C in (([50, 31], 32), ([50, 31], 10), ([3000], 512)):
+        M = sum(lengths) + 2
+        rows = P.PackedRows.from_offsets(offsets(lengths), M)
+        x, g, got = randn(M, C, seed=1), randn(M, C, seed=2), []
+        for needs in (True, False):
+            w, b = torch.nn.Parameter(randn(C, seed=3)), torch.nn.Parameter(randn(C, seed=4))
+            P.group_norm(x.clone().requires_grad_(needs), w, b, 2, rows, 1e-5, "silu").backward(g)
+            got.append((w.grad, b.grad))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@gpu
+def test_group_norm_backward_captured_beside_a_living_eager_graph():
+    """the parameters have no autograd node: an eager result that still holds its graph does not reach into the capture"""
+    from optispeech_amd import packed_ops as P
+    lengths, C = [60, 41], 64
+    rows = P.PackedRows.from_offsets(offsets(lengths), 101)
+    x, g = randn(101, C, seed=1), randn(101, C, seed=2)
+    w, b = torch.nn.Parameter(randn(C, seed=3)), torch.nn.Parameter(randn(C, seed=4))
+    w.grad, b.grad = torch.zeros_like(w), torch.zeros_like(b)
+    alive = P.group_norm(x, w, b, 4, rows, 1e-5, "silu")
+
+    def step():
+        w.grad.zero_(), b.grad.zero_()
+        y = P.group_norm(x, w, b, 4, rows, 1e-5, "silu")
+        y.backward(g)
+        return y.detach()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    for i in range(3):
+        x.copy_(randn(101, C, seed=10 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [y.clone(), w.grad.clone(), b.grad.clone()]
+        for a, e in zip(got, (step(), w.grad, b.grad)):
+            assert torch.equal(a, e)
+    assert alive.grad_fn is not None
+
+
+@gpu
+@pytest.mark.parametrize("started", [False, True])
+def test_group_norm_one_parameter_as_weight_and_bias(started):
+    """its gradient is the sum of both; ``started``: a gradient is there already.  Each gradient is rounded once and so is every sum: the same
+    operations as with two parameters, in the same order"""
+    from optispeech_amd import packed_ops as P
+    for lengths, C in (([50, 31], 32), ([50, 31], 10)):
+        M = sum(lengths)
+        rows = P.PackedRows.from_offsets(offsets(lengths), M)
+        x, g = randn(M, C, seed=1).requires_grad_(), randn(M, C, seed=2)
+        p, w, b = (torch.nn.Parameter(randn(C, seed=3)) for _ in range(3))
+        had = randn(C, seed=5) if started else torch.zeros(C, device=DEV)
+        if started:
+            p.grad = had.clone()
+        P.group_norm(x, p, p, 2, rows).backward(g)
+        P.group_norm(x, w, b, 2, rows).backward(g)
+        assert torch.equal(p.grad, w.grad + (b.grad + had))
+
+
+@gpu
+def test_rotary_of_broadcast_heads_and_rows():
+    """heads and rows of stride 0 are read in place; their gradient is the sum over the copies, as autograd forms it"""
+    from optispeech_amd import packed_ops as P
+    lengths, D = [9, 4], 16
+    M = sum(lengths)
+    rows, rope = P.PackedRows.from_offsets(offsets(lengths), M), P.Rotary(D)
+    for shape, size in (((M, 1, D), (M, 3, D)), ((1, 3, D), (M, 3, D)), ((1, 1, D), (M, 3, D))):
+        t, g = randn(*shape, seed=1), randn(M, 3, D, seed=2)
+        a, b = t.clone().requires_grad_(), t.clone().requires_grad_()
+        ya, yb = P.rotary(a.expand(size), g, rope, rows)[0], P.rotary(b.expand(size).contiguous(), g, rope, rows)[0]
+        assert torch.equal(ya, yb)
+        assert torch.equal(torch.autograd.grad(ya, (a,), g)[0], torch.autograd.grad(yb, (b,), g)[0])
+
+
+@gpu
+def test_refused_sizes():
+    from optispeech_amd import packed_ops as P
+    from optispeech_amd._lib import OspError
+    with pytest.raises(OspError, match="rows"):
+        P.PackedRows.from_offsets(offsets([1]), 2 ** 31 - 65535)
+    wide = torch.zeros(1, 1, 1, device=DEV, dtype=torch.bfloat16).expand(1, 65536, 2048)       # 2^27 channels in a row
+    with pytest.raises(OspError, match="channels"):
+        P.rotary(wide, wide[:, :1], P.Rotary(8), P.PackedRows.from_offsets(offsets([1]), 1))
 
 
 @gpu
