@@ -131,12 +131,12 @@ class ConvolutionModule(nn.Module):
         self.norm_groups = norm_groups
         self.pointwise_conv2 = _Conv1dK1(channels, channels)
 
-    def forward(self, x, rows=None, valid=None):
+    def forward(self, x, rows=None, pad=None):
         C = x.shape[-1]
         u = self.pointwise_conv1(x)
         u = u[..., :C] * torch.sigmoid(u[..., C:])                                               # GLU over the channel pairs
         if self.norm_groups is not None:                          # padded frames stay out of the convolution and of the statistics
-            return self.pointwise_conv2(self.norm(self.depthwise_conv((u * valid).contiguous()), rows))
+            return self.pointwise_conv2(self.norm(self.depthwise_conv(u.masked_fill(pad, 0.0).contiguous()), rows))
         u = self.norm(self.depthwise_conv(u.contiguous()))
         return self.pointwise_conv2(u * torch.sigmoid(u))                                        # swish
 
@@ -158,14 +158,14 @@ class EncoderLayer(nn.Module):
             y = y * scale
         return ops.dropout_add(y, self.dropout_rate, self.training, self._s[i], res=x)
 
-    def forward(self, x, pos_emb, klen, rows=None, valid=None):
+    def forward(self, x, pos_emb, klen, rows=None, pad=None):
         x = self._res(x, self.feed_forward_macaron(self.norm_ff_macaron(x)), 0, 0.5)
         if rows is None:
             x = self._res(x, self.self_attn(self.norm_mha(x), pos_emb, klen), 1)
             x = self._res(x, self.conv_module(self.norm_conv(x)), 2)
         else:
             x = self._res(x, self.self_attn(self.norm_mha(x), rows), 1)
-            x = self._res(x, self.conv_module(self.norm_conv(x), rows, valid), 2)
+            x = self._res(x, self.conv_module(self.norm_conv(x), rows, pad), 2)
         x = self._res(x, self.feed_forward(self.norm_ff(x)), 3, 0.5)
         return self.norm_final(x)
 
@@ -198,9 +198,9 @@ class Encoder(nn.Module):
         if self.packed:
             from ..packed_ops import PackedRows
             rows = PackedRows.from_padded(klen, T)
-            valid = (torch.arange(T, device=xs.device)[None] < klen[:, None])[:, :, None].to(xs.dtype)
+            pad = (torch.arange(T, device=xs.device)[None] >= klen[:, None])[:, :, None]
             for layer in self.encoders:
-                xs = layer(xs, None, None, rows, valid)
+                xs = layer(xs, None, None, rows, pad)
             return self.after_norm(xs)
         pos = rel_positions(T, self.d, xs.device)
         if self.training and self.pos_drop > 0.0 and (2 * T - 1) * self.d % 4 == 0:

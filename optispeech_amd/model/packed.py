@@ -65,8 +65,12 @@ class FrameCache:
 
     def begin(self, frames):
         """rows of the next ``frames`` frames of every stream"""
+        if frames < 1:
+            raise P.OspError(f"{frames} new frames")
         if self.used + frames > self.capacity:
             raise P.OspError(f"{self.used} + {frames} frames in a cache of {self.capacity}")
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():      # replays would pass the capacity unseen
+            raise P.OspError("a stream's step counts its frames on the host: it cannot be captured into a graph")
         dev = self.length.device
         self._rows = P.PackedRows.from_offsets(torch.arange(0, (self.streams + 1) * frames, frames, device=dev), self.streams * frames, longest=frames)
         self._keys = P.PackedRows.from_padded(self.length + frames, self.capacity)

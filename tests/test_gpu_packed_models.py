@@ -186,6 +186,31 @@ def test_conformer_utterances_do_not_see_their_padding(mode, tol):
 
 
 @gpu
+@pytest.mark.parametrize("mode", ["f32", "bf16"])
+def test_padding_may_hold_nan(mode):
+    """valid frames do not depend on what the padding holds, NaN included"""
+    from optispeech_amd import precision
+    from optispeech_amd.model.conformer import Conformer
+    precision.set_precision(mode)
+    try:
+        torch.manual_seed(4)
+        conformer = Conformer(dim=64, attention_heads=2, linear_units=96, num_blocks=2, attention_dropout_rate=0.0, selfattention_layer_type="packed",
+                              cnn_module_norm_groups=4).to(DEV).eval()
+        lens, T = [33, 1, 20], 33
+        x = torch.randn(3, T, 64, generator=torch.Generator().manual_seed(6)).to(DEV)
+        pad = (torch.arange(T)[None] >= torch.tensor(lens)[:, None]).to(DEV)
+        for m in (conformer, make_transformer(causal=True)):
+            got = []
+            for fill in (0.0, float("nan")):
+                x[pad] = fill
+                with torch.no_grad():
+                    got.append(m(x, pad)[~pad])
+            assert torch.isfinite(got[0]).all() and torch.equal(got[0], got[1])
+    finally:
+        precision.set_precision("f32")
+
+
+@gpu
 @pytest.mark.parametrize("backbone", ["transformer", "conformer"])
 @pytest.mark.parametrize("mode", ["bf16", "f32"])
 def test_training_step_with_the_packed_attention(backbone, mode):
@@ -234,3 +259,17 @@ def test_refusals():
     cache = FrameCache(1, 2, 4, 1, 8, "cpu", torch.float32)
     with pytest.raises(OspError, match="cache"):
         cache.begin(5)
+
+
+def test_stream_refusals(monkeypatch):
+    """steps of no frames, and steps inside a capture, whose replays would not be counted"""
+    from optispeech_amd.model.packed import FrameCache
+    from optispeech_amd._lib import OspError
+    cache = FrameCache(1, 2, 4, 1, 8, "cpu", torch.float32)
+    with pytest.raises(OspError, match="0 new frames"):
+        cache.begin(0)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(OspError, match="captured"):
+        cache.begin(1)
+    assert cache.used == 0
