@@ -55,7 +55,8 @@ class PackedRows:
             raise OspError("offsets / lengths must live on the GPU")
         if docs < 1 or rows < 0 or longest < 0:
             raise OspError(f"a batch needs at least one document (docs {docs}, rows {rows}, longest {longest})")
-        self.docs, self.rows, self.longest, self.device = docs, rows, min(longest, rows), src.device
+        # (a bound chooses kernels and splits, never results: one of 0 counts as 1, the documents may have rows all the same)
+        self.docs, self.rows, self.longest, self.device = docs, rows, min(max(longest, 1), rows), src.device
         self.cap = _size("osp_packed_rows_tiles", docs, rows)
         long = torch.empty((2, docs), device=src.device, dtype=torch.int64)
         self._buffers, self._stream = [long], _lib._raw_stream(src.device.index)
@@ -215,12 +216,10 @@ def _normalise(x, w, b, groups, rows, eps, act):
     M, C = x.shape
     y = torch.empty((M, C), device=x.device, dtype=x.dtype)
     stats = torch.empty((2, rows.docs, groups), device=x.device, dtype=torch.float32)
-    if M and rows.longest:
+    if M:
         ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 0), x.device)
         call("osp_group_norm_fwd", x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, y, stats, ws, rows.begin, rows.length, rows.base, rows.tiles,
              rows.ntiles, rows.cap, rows.docs, M, rows.longest, C, groups, eps, act)
-    else:
-        y.zero_()
     return x, y, stats
 
 
@@ -253,7 +252,7 @@ class GroupNormFn(torch.autograd.Function):
         dx = torch.empty((M, C), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
         db, add_b = _grad_target(b)                                # the kernels write db first, then dw: one tensor may be both
         dw, add_w = _grad_target(w)
-        if M and rows.longest:
+        if M:
             ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 1), x.device)
             call("osp_group_norm_bwd", dy, dy.stride(0), x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, stats, dx, dw, add_w, db, add_b, ws,
                  rows.begin, rows.length, rows.base, rows.tiles, rows.ntiles, rows.cap, rows.docs, M, rows.longest, C, groups, act)
