@@ -156,14 +156,15 @@ def _rotate(q, k, rope, rows, first, out_dtype, inverse):
 class RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, rope, rows, first, out_dtype):
-        ctx.cfg = (rope, rows, first, q.dtype)
+        ctx.save_for_backward(first)                               # (its values at this call: a counter advanced in place is noticed)
+        ctx.cfg = (rope, rows, q.dtype)
         ctx.shapes = (q.shape, k.shape, out_dtype, q.device)
         return _rotate(q, k, rope, rows, first, out_dtype, False)
 
     @staticmethod
     def backward(ctx, dq, dk):
         _first_order()
-        rope, rows, first, dtype = ctx.cfg
+        (first,), (rope, rows, dtype) = ctx.saved_tensors, ctx.cfg
         qs, ks, od, dev = ctx.shapes
         dq = torch.zeros(qs, device=dev, dtype=od) if dq is None else dq.to(od)
         dk = torch.zeros(ks, device=dev, dtype=od) if dk is None else dk.to(od)

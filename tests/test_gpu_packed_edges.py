@@ -36,3 +36,19 @@ def test_a_bound_of_no_rows_costs_time_and_not_results(dtype):
         scale = a.double().abs().max().item()
         assert scale > 0.1 and float((a.double() - b.double()).abs().max()) <= (torch.finfo(a.dtype).eps + 150 * U * (30 if i >= 2 else 1)) * scale
     assert all(torch.equal(a, b) for a, b in zip(*turned))
+
+
+@gpu
+def test_rotary_positions_advanced_before_the_backward_are_refused():
+    """`first` belongs to the call: a counter advanced in place between forward and backward raises, as for any tensor that autograd keeps"""
+    from optispeech_amd import packed_ops as P
+    rows = P.PackedRows.from_offsets(offsets([3, 2]), 5)
+    q, k, g = (randn(5, 2, 16, seed=i).requires_grad_() for i in range(3))
+    first = torch.tensor([7, 100], dtype=torch.int64, device=DEV)
+    rope = P.Rotary(16)
+    yq, yk = P.rotary(q, k, rope, rows, first=first)
+    first += 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad((yq, yk), (q, k), (g, g))
+    yq, yk = P.rotary(q, k, rope, rows, first=first)
+    torch.autograd.grad((yq, yk), (q, k), (g, g))
