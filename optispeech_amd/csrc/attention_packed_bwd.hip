@@ -521,7 +521,7 @@ KeyPlan plan_keys(int64_t rows, int64_t docs, int64_t Hk, int64_t G, int64_t qlo
 
 template <typename T, int DP>
 void launch(Args p, const PackedTile* ktiles, const int* kntiles, int kcap, hipStream_t s) {
-    const int mode = (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0);
+    const int mode = score_mode(p, sizeof(T) == 2);
     Args pk = p;
     pk.tiles = ktiles; pk.ntiles = kntiles; pk.cap_tiles = kcap;
     const bool sq = split_waves(p.Mq, p.docs, p.Hq, p.klongest, sizeof(T) == 4, DP > 64), sk = plan_keys(p.Mk, p.docs, p.Hk, p.G, p.qlongest, p.D, sizeof(T) == 4).split;
@@ -531,7 +531,10 @@ void launch(Args p, const PackedTile* ktiles, const int* kntiles, int kcap, hipS
     else hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, M_>), gq, dim3(256), 0, s, p);             \
     if (sk) hipLaunchKernelGGL((packed_attn_dkv_split_kernel<T, DP, M_>), gk, dim3(256), 0, s, pk);  \
     else hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, M_>), gk, dim3(256), 0, s, pk)
-    if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else { L(3); }
+    if constexpr (sizeof(T) == 2) {
+        if (mode == (CAP | WIDE)) { L(CAP | WIDE); } else if (mode == (CAP | SLOPE | WIDE)) { L(CAP | SLOPE | WIDE); }
+    }
+    if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else if (mode == 3) { L(3); }
 #undef L
     if (p.parts > 1) hipLaunchKernelGGL((packed_attn_parts_kernel<T>), dim3((unsigned)kcap, 2, 4), dim3(256), 0, s, pk);
 }

@@ -27,7 +27,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float EMPTY = 1.0e30f;             // log-sum-exp of a query that sees nothing: exp2(s - EMPTY) = 0
 constexpr float NONE = -1.0e30f;             // running maximum before the first seen key
 
-enum { CAP = 1, SLOPE = 2 };                 // score function of an instantiation
+enum { CAP = 1, SLOPE = 2, WIDE = 4 };       // score function of an instantiation; WIDE (with CAP, bf16 tensors): a cap above WIDE_CAP
+constexpr float WIDE_CAP = 512.f;
 
 struct Args {
     const void *q, *k, *v, *o, *dout;
@@ -212,17 +213,21 @@ __device__ __forceinline__ f32x16 splat(float v) {
 
 // The score function of a raw product x = q . k (scale > 0), in log2 units, as  s = a u + b:
 //   plain: u = x, a = scale log2 e;   cap: u = -1 / (exp(2 y) + 1) with y = scale x / cap, a = 2 cap log2 e, b = cap log2 e  (cap tanh y = cap - 2 cap / (exp
-//   2 y + 1) on v_exp_f32 and v_rcp_f32: off by 2^-22 of the cap at most);  EXACT (f32 tensors): u = tanh y by the library, a = cap log2 e
+//   2 y + 1) on v_exp_f32 and v_rcp_f32: off by 2^-22 of the cap at most);  EXACT (f32 tensors) and WIDE: u = tanh y by the library, a = cap log2 e, whose
+//   error is relative to the score.  WIDE starts at a cap of 512, where the first form is off by 1.2e-4 (a probability's rounding to bf16: 2e-3); on
+//   either side of it (caps 512 and 513, causal): 4 x 4096 rows, 16 heads of 128 sharing 4: forward 358 and 430 us, training 1.69 and 2.26 ms;  24 x 700 rows,
+//   8 heads of 64: 36 and 50 us, 143 and 192 us;  48 new tokens over 8192 keys each: 92 us both
 //   slope: u becomes the score itself with the distance's penalty, a = 1, b = 0
 // A maximum over u is a maximum over s, and a u + b - max is one FMA in front of the exponential.
 // The cap's derivative 1 - tanh^2 y is 4 (-u - u u) for the first form: the factor 4 goes to the caller (grad_scale).
 template <int MODE, bool EXACT>
 struct Score {
+    static constexpr bool LIB = EXACT || (MODE & WIDE);
     float c1, a, b, fa, fb, slope2;
     __device__ __forceinline__ Score(const Args& p, int head) {
         c1 = 0.f; slope2 = 0.f;
         if constexpr (!(MODE & CAP)) { a = p.scale * LOG2E; b = 0.f; }
-        else if constexpr (EXACT) { c1 = p.scale / p.softcap; a = p.softcap * LOG2E; b = 0.f; }
+        else if constexpr (LIB) { c1 = p.scale / p.softcap; a = p.softcap * LOG2E; b = 0.f; }
         else { c1 = 2.f * p.scale * LOG2E / p.softcap; a = 2.f * p.softcap * LOG2E; b = p.softcap * LOG2E; }
         fa = a; fb = b;
         if constexpr (MODE & SLOPE) { fa = 1.f; fb = 0.f; }
@@ -231,7 +236,7 @@ struct Score {
     __device__ __forceinline__ void set_head(const Args& p, int head) { if constexpr (MODE & SLOPE) slope2 = p.slopes[head] * LOG2E; }
     __device__ __forceinline__ float cap(float x) const {
         if constexpr (!(MODE & CAP)) return x;
-        if constexpr (EXACT) return tanhf(x * c1);
+        if constexpr (LIB) return tanhf(x * c1);
         return -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f);
     }
     __device__ __forceinline__ float penalise(float u, float distance) const {
@@ -239,8 +244,8 @@ struct Score {
         return u;
     }
     // derivative of the capped score by the raw one, from cap(x), without grad_scale
-    __device__ __forceinline__ float derive(float c) const { return EXACT ? fmaf(-c, c, 1.f) : fmaf(-c, c, -c); }
-    static constexpr float grad_scale = (MODE & CAP) && !EXACT ? 4.f : 1.f;
+    __device__ __forceinline__ float derive(float c) const { return LIB ? fmaf(-c, c, 1.f) : fmaf(-c, c, -c); }
+    static constexpr float grad_scale = (MODE & CAP) && !LIB ? 4.f : 1.f;
 };
 
 // host: too few tiles of 128 rows (of `heads` heads) to fill the chip: the waves of a workgroup share 32 rows instead of owning 32 each.  `path`: rows a
@@ -254,6 +259,11 @@ static inline bool split_waves(int64_t rows, int64_t docs, int64_t heads, int64_
     if (f32) return n < (path >= 512 ? 384 : 192);
     if (narrow_limit) return n < 72;                     // gradients of wide bf16 heads: the private tiles cost occupancy
     return n < (path >= 2048 ? 384 : 128);
+}
+
+// host: the score function of a call
+static inline int score_mode(const Args& p, bool bf16) {
+    return (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0) | (bf16 && p.softcap > WIDE_CAP ? WIDE : 0);
 }
 
 // host: a tile's rows fit a buffer descriptor, and a row reaches no further than the next

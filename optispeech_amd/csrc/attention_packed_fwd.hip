@@ -278,13 +278,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void packed_attn_fwd_s
 
 template <typename T, int DP, bool FINE>
 void launch(const Args& p, hipStream_t s) {
-    const int mode = (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0);
+    const int mode = score_mode(p, sizeof(T) == 2);
     const bool split = split_waves(p.Mq, p.docs, p.Hq, p.klongest, sizeof(T) == 4, false);
     const dim3 grid((unsigned)(p.cap_tiles * p.Hq * (split ? 4 : 1)));
 #define L(M_)                                                                                                        \
     if (split) hipLaunchKernelGGL((packed_attn_fwd_split_kernel<T, DP, M_, FINE>), grid, dim3(256), 0, s, p);        \
     else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, M_, FINE>), grid, dim3(256), 0, s, p)
-    if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else { L(3); }
+    if constexpr (sizeof(T) == 2) {
+        if (mode == (CAP | WIDE)) { L(CAP | WIDE); } else if (mode == (CAP | SLOPE | WIDE)) { L(CAP | SLOPE | WIDE); }
+    }
+    if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else if (mode == 3) { L(3); }
 #undef L
 }
 template <typename T, bool FINE>

@@ -189,9 +189,12 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const Args p, int
 template <typename T, int DP>
 void launch(const Args& p, int B, int chunk, int nsplit, float* po, float* pm, hipStream_t s) {
     const dim3 grid((unsigned)nsplit, (unsigned)p.Hk, (unsigned)B);
-    const int mode = (p.softcap > 0.f ? CAP : 0) | (p.slopes ? SLOPE : 0);
+    const int mode = score_mode(p, sizeof(T) == 2);
 #define L(M_) hipLaunchKernelGGL((packed_attn_token_kernel<T, DP, M_>), grid, dim3(256), 0, s, p, chunk, nsplit, po, pm)
-    if (mode == 0) L(0); else if (mode == 1) L(1); else if (mode == 2) L(2); else L(3);
+    if constexpr (sizeof(T) == 2) {
+        if (mode == (CAP | WIDE)) { L(CAP | WIDE); } else if (mode == (CAP | SLOPE | WIDE)) { L(CAP | SLOPE | WIDE); }
+    }
+    if (mode == 0) { L(0); } else if (mode == 1) { L(1); } else if (mode == 2) { L(2); } else if (mode == 3) { L(3); }
 #undef L
     hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)p.cap_tiles, (unsigned)p.Hq), dim3(256), 0, s, p, chunk, nsplit, po, pm);
 }

@@ -52,3 +52,42 @@ def test_rotary_positions_advanced_before_the_backward_are_refused():
         torch.autograd.grad((yq, yk), (q, k), (g, g))
     yq, yk = P.rotary(q, k, rope, rows, first=first)
     torch.autograd.grad((yq, yk), (q, k), (g, g))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cap", [512.0, 600.0, 1e5, 1e7, 1e12, 1e20])
+@pytest.mark.parametrize("slope", [False, True])
+@pytest.mark.parametrize("lengths,H,S,D", [([300, 40], 4, 2, 64), ([129] * 40, 8, 4, 128), ([33, 5], 2, 2, 32)])
+def test_caps_far_above_the_scores(dtype, cap, slope, lengths, H, S, D):
+    """A cap far above the scores leaves them as they are, and with the accuracy of uncapped ones.  The bound is the uncapped one: the tanh's form adds to a score s
+    at most 8 u |s| above 512 (scale / cap, its product, tanhf 2 ulp = 4 u, the product with cap log2 e and its rounding) and 16 u 512 = 8192 u up to there
+    (stated separately); (D + 8) u sum |q k| grows to (D + 16) u: a factor of at most 1.2 for D >= 32."""
+    from optispeech_amd import packed_ops as P
+    M = sum(lengths)
+    q, do = randn(M, H, D, seed=1, dtype=dtype), randn(M, H, D, seed=4, dtype=dtype)
+    k, v = randn(M, S, D, seed=2, dtype=dtype), randn(M, S, D, seed=3, dtype=dtype)
+    slopes = torch.tensor([0.5 ** (h + 1) for h in range(H)], device=DEV) if slope else None
+    rows = P.PackedRows.from_offsets(offsets(lengths), M, longest=max(lengths))
+    docs = ref.documents(lengths)
+    want, tol = bounds(q, k, v, do, docs, docs, D ** -0.5, True, None, cap, slopes, dtype)
+    if cap > 512 or dtype == torch.float32:
+        tol = [1.25 * t for t in bounds(q, k, v, do, docs, docs, D ** -0.5, True, None, 0.0, slopes, dtype)[1]]
+    close(grads(q, k, v, do, rows, causal=True, softcap=cap, slopes=slopes), want, tol)
+    # a new token over the same keys
+    B = len(lengths)
+    last = torch.tensor([sum(lengths[:i + 1]) - 1 for i in range(B)], device=DEV)
+    o = P.attention(q[last], k, v, P.PackedRows.from_offsets(offsets([1] * B), B, longest=1), keys=rows, causal=True, softcap=cap, slopes=slopes)
+    close((o,), (want[0][last.cpu()],), (tol[0][last.cpu()],))
+
+
+@gpu
+def test_caps_out_of_range_are_refused():
+    """scale / cap has to be an ordinary f32 number"""
+    from optispeech_amd import packed_ops as P
+    from optispeech_amd._lib import OspError
+    h = torch.zeros(4, 4, 8, device=DEV)
+    rows = P.PackedRows.from_offsets(offsets([4]), 4)
+    for cap in (1e-40, 1e-31, 1e31, 1e38, 1e300):
+        with pytest.raises(OspError, match="softcap"):
+            P.attention(h, h, h, rows, softcap=cap, scale=1.0)
