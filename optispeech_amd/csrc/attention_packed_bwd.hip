@@ -33,11 +33,11 @@ __device__ __forceinline__ void dq_block(f32x16 (&acc)[DP / 32], const char* kt,
     for (int i = 0; i < 16; ++i) {
         const int r = (i >> 2) * 8 + (i & 3);
         const float c = sc.cap(st[i]);
-        float pr = __builtin_amdgcn_exp2f(fmaf(sc.penalise(c, dist - (float)r), sc.fa, shift));
-        if constexpr (MASKED) pr = r < left ? pr : 0.f;
         float d = dp[i];
         if constexpr (MODE & CAP) d *= sc.derive(c);
-        O::set(ds, i, pr * d);
+        d *= __builtin_amdgcn_exp2f(fmaf(sc.penalise(c, dist - (float)r), sc.fa, shift));
+        if constexpr (MASKED) d = r < left ? d : 0.f;                                  // the product: a query that sees nothing may hold NaN, in dO too
+        O::set(ds, i, d);
     }
     O::template value<DP>(acc, ds, kt, lane);
 }

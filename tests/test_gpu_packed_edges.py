@@ -91,3 +91,28 @@ def test_caps_out_of_range_are_refused():
     for cap in (1e-40, 1e-31, 1e31, 1e38, 1e300):
         with pytest.raises(OspError, match="softcap"):
             P.attention(h, h, h, rows, softcap=cap, scale=1.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cap,slope", [(0.0, False), (9.0, True)])
+@pytest.mark.parametrize("pairs,H,S,D", [([(40, 10), (5, 5)], 2, 1, 64), ([(140, 70), (200, 129), (33, 0), (12, 12)] * 15, 12, 4, 128)])
+def test_queries_that_see_nothing_may_hold_nan(dtype, cap, slope, pairs, H, S, D):
+    """causal, more queries than keys: the first queries see nothing.  Whatever they and their incoming gradient hold, they get zeros and the others get
+    what they get without them, bit for bit"""
+    from optispeech_amd import packed_ops as P
+    qlens, klens = zip(*pairs)
+    M, Mk = sum(qlens), sum(klens)
+    q, do = randn(M, H, D, seed=1, dtype=dtype), randn(M, H, D, seed=4, dtype=dtype)
+    k, v = randn(Mk, S, D, seed=2, dtype=dtype), randn(Mk, S, D, seed=3, dtype=dtype)
+    rows = P.PackedRows.from_offsets(offsets(qlens), M, longest=max(qlens))
+    keys = P.PackedRows.from_offsets(offsets(klens), Mk, longest=max(klens))
+    blind = torch.cat([torch.arange(nq) < nq - nk for nq, nk in pairs]).to(DEV)
+    slopes = torch.tensor([0.5 ** (h + 1) for h in range(H)], device=DEV) if slope else None
+    out = []
+    for fill in (0.0, float("nan")):
+        q[blind], do[blind] = fill, fill
+        out.append(grads(q, k, v, do, rows, keys=keys, causal=True, softcap=cap, slopes=slopes))
+    for a, b in zip(*out):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    assert float(out[1][0][blind].detach().abs().max()) == 0.0 and float(out[1][1][blind].abs().max()) == 0.0
