@@ -299,7 +299,7 @@ int osp_conv_gemm_f32_split(const float* A, int64_t lda, int64_t M, int64_t T, i
 /* replaces: workspace query for osp_group_norm_fwd / osp_group_norm_bwd */
 int64_t osp_group_norm_workspace_bytes(int64_t B, int64_t M, int64_t C, int64_t G, int64_t backward);
 
-/* replaces: no reference counterpart: group norm + activation over the rows of each document (the place of BatchNorm + swish in _conformer/convolution.py:61-70, which counts padded frames) */
+/* replaces: no reference counterpart: group norm + activation over the rows of each document (the place of BatchNorm + swish in _conformer/convolution.py:61-70, which counts padded frames); stats: (3, B, G) f32, mean, 1 / deviation and the mean's part below f32 */
 int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, const float* w, const float* b, void* y, float* stats, void* workspace, const int64_t* begin, const int64_t* len, const int32_t* base, const int32_t* tiles, const int32_t* ntiles, int64_t cap, int64_t B, int64_t M, int64_t longest, int64_t C, int64_t G, float eps, int64_t act, hipStream_t stream);
 
 /* replaces: autograd of the same */

@@ -52,7 +52,7 @@ extern "C" int osp_kernel_note_bytes_host(double* bytes_host) {
 // ABI history: 1 = rounds 1-2; 2 = round 3 added trailing workspace parameters to osp_layernorm_bwd / osp_ln_dwconv7_bwd /
 // osp_smallcin_conv_wgrad (a consumer built against the version-1 header would pass its stream in the workspace slot) and round 4
 // added osp_memset / osp_copy / osp_store_i64 / the fused block entry points.  Bump whenever an EXISTING signature changes.
-extern "C" int osp_abi_version() { return 2; }
+extern "C" int osp_abi_version() { return 3; }
 
 // Content hash of the sources (and flags) this library was compiled from: optispeech_amd/build.py passes it on the command line
 // of this file and compares it with the sources next to a shipped library (the marker prefix makes it findable without dlopen).

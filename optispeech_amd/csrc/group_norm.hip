@@ -5,8 +5,10 @@
 //             dw += sum dz xhat,  db += sum dz   over all documents
 // Rows of no document get zeros (y and dx) and add nothing.
 //
-// Sums: x and x^2 are summed in 64 bits (x^2 of an f32 is exact there, so a mean far above the deviation costs nothing; the vector units
-// do 64-bit FMAs at the 32-bit rate and the kernel is bound by HBM).  The backward's per-channel sums run in 32 bits over the rows of one
+// Sums: x and x^2 are summed in 64 bits (x^2 of an f32 is exact there; the vector units do 64-bit FMAs at the 32-bit rate and the kernel is bound by HBM),
+// and for f32 tensors the mean is kept as two floats, m + rest: rounded to one it would shift every xhat of a group by up to 2^-24 |mean| / deviation.  A
+// mean far above the deviation then costs what the 64-bit sums lose, about 2^-53 (mean / deviation)^2 of rstd per addition in a chain (1e-6 where
+// the mean is 10^5 deviations), instead of 6e-3.  The backward's per-channel sums run in 32 bits over the rows of one
 // workgroup (at most PACKED_TILE) and in 64 bits from there on.  Every sum has one fixed order: no atomics.
 //
 // Bound: HBM.  Where a document's rows x one slab of groups fit the registers of a workgroup, one launch reads x (and dy) once: see "documents that fit".
@@ -58,7 +60,7 @@ struct NormArgs {
     const void* dy; int64_t lddy;
     const float *w, *b;
     void* out;                                  // y or dx, (M, C) contiguous
-    float *mean, *rstd;                         // (B, G)
+    float *mean, *rstd, *rest;                  // (B, G); rest: the mean's part below f32, for f32 tensors
     double* part;                               // forward: (slots, G, 2)
     float* cpart;                               // backward: (slots, C, 2)
     double* dsum;                               // backward: (B, C, 2) sums of dz, dz xhat
@@ -99,8 +101,15 @@ __device__ __forceinline__ double lane_group_sum(double v, int L) {
     return v;
 }
 
-// a document's statistics from its partials; results for every group in LDS
-__device__ __forceinline__ void doc_stats(const NormArgs& p, int doc, int64_t rows, float* mean_l, float* rstd_l) {
+// x - mean: f32 tensors take the mean's second part off too (bf16 values resolve 2^-9 of the mean: its rounding to f32 is far below)
+template <typename T>
+__device__ __forceinline__ float centre(float x, float m, float rest) {
+    if constexpr (sizeof(T) == 4) return (x - m) - rest;
+    return x - m;
+}
+
+// a document's statistics from its partials; results for every group in LDS: G means, G rstd, G rests
+__device__ __forceinline__ void doc_stats(const NormArgs& p, int doc, int64_t rows, float* stat_l) {
     const int nslots = (int)((rows + PACKED_TILE - 1) / PACKED_TILE) * p.sub;
     const double* part = p.part + (int64_t)p.base[doc] * p.sub * p.G * 2;
     int L = 1;
@@ -118,8 +127,9 @@ __device__ __forceinline__ void doc_stats(const NormArgs& p, int doc, int64_t ro
         q = lane_group_sum(q, L);
         if (g < p.G && l == 0) {
             const double m = s / count, var = fmax(q / count - m * m, 0.0);
-            mean_l[g] = (float)m;
-            rstd_l[g] = (float)(1.0 / sqrt(var + (double)p.eps));
+            stat_l[g] = (float)m;
+            stat_l[p.G + g] = (float)(1.0 / sqrt(var + (double)p.eps));
+            stat_l[2 * p.G + g] = (float)(m - (double)(float)m);
         }
     }
     __syncthreads();
@@ -178,22 +188,26 @@ __global__ __launch_bounds__(NTH) void gn_stats_kernel(const NormArgs p) {
 
 // statistics of one document per workgroup (where a document has too many partials for every apply workgroup to add them)
 __global__ __launch_bounds__(NTH) void gn_finish_kernel(const NormArgs p) {
-    __shared__ float mean_l[MAXC], rstd_l[MAXC];
+    __shared__ float stat_l[3 * MAXC];
     const int doc = blockIdx.x;
     const int64_t rows = p.len[doc];
     if (rows <= 0) {
-        for (int g = threadIdx.x; g < p.G; g += NTH) { p.mean[(int64_t)doc * p.G + g] = 0.f; p.rstd[(int64_t)doc * p.G + g] = 0.f; }
+        for (int g = threadIdx.x; g < p.G; g += NTH) { p.mean[(int64_t)doc * p.G + g] = 0.f; p.rstd[(int64_t)doc * p.G + g] = 0.f; p.rest[(int64_t)doc * p.G + g] = 0.f; }
         return;
     }
-    doc_stats(p, doc, rows, mean_l, rstd_l);
-    for (int g = threadIdx.x; g < p.G; g += NTH) { p.mean[(int64_t)doc * p.G + g] = mean_l[g]; p.rstd[(int64_t)doc * p.G + g] = rstd_l[g]; }
+    doc_stats(p, doc, rows, stat_l);
+    for (int g = threadIdx.x; g < p.G; g += NTH) {
+        p.mean[(int64_t)doc * p.G + g] = stat_l[g];
+        p.rstd[(int64_t)doc * p.G + g] = stat_l[p.G + g];
+        p.rest[(int64_t)doc * p.G + g] = stat_l[2 * p.G + g];
+    }
 }
 
 
 // ------------------------------------------------------------------------------------------------ forward: apply
 template <typename T, int V, int ACT, bool DIRECT>
 __global__ __launch_bounds__(NTH) void gn_apply_kernel(const NormArgs p) {
-    extern __shared__ float stat[];             // [G] mean, [G] rstd
+    extern __shared__ float stat[];             // [G] mean, [G] rstd, [G] rest
     if ((int)blockIdx.x >= p.ntiles[1]) return;
     const PackedTile tile = p.tiles[blockIdx.x];
     const int step = PACKED_TILE / p.sub, lo = blockIdx.y * step, hi = min(tile.n, lo + step);
@@ -201,31 +215,33 @@ __global__ __launch_bounds__(NTH) void gn_apply_kernel(const NormArgs p) {
     T* y = reinterpret_cast<T*>(p.out) + (int64_t)tile.row0 * p.C;
     if (tile.doc < 0) { zero_rows(y + (int64_t)lo * p.C, (int64_t)(hi - lo) * p.C); return; }
     if (DIRECT) {
-        doc_stats(p, tile.doc, p.len[tile.doc], stat, stat + p.G);
+        doc_stats(p, tile.doc, p.len[tile.doc], stat);
         if (tile.i0 == 0 && lo == 0)
             for (int g = threadIdx.x; g < p.G; g += NTH) {
                 p.mean[(int64_t)tile.doc * p.G + g] = stat[g];
                 p.rstd[(int64_t)tile.doc * p.G + g] = stat[p.G + g];
+                p.rest[(int64_t)tile.doc * p.G + g] = stat[2 * p.G + g];
             }
     }
     const float* mean = DIRECT ? stat : p.mean + (int64_t)tile.doc * p.G;
     const float* rstd = DIRECT ? stat + p.G : p.rstd + (int64_t)tile.doc * p.G;
+    const float* rest = DIRECT ? stat + 2 * p.G : p.rest + (int64_t)tile.doc * p.G;
     const Lanes l = lanes_of(p.C / V);
     const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row0 * p.ldx;
     const int cg = p.C / p.G;
     for (int cv = l.cx; cv < p.C / V && l.ry < l.ny; cv += l.nx) {
-        float m[V], rs[V], w[V], b[V];
+        float m[V], rs[V], ml[V], w[V], b[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = cv * V + i, g = c / cg;
-            m[i] = mean[g]; rs[i] = rstd[g]; w[i] = p.w[c]; b[i] = p.b[c];
+            m[i] = mean[g]; rs[i] = rstd[g]; ml[i] = rest[g]; w[i] = p.w[c]; b[i] = p.b[c];
         }
 #pragma unroll 4
         for (int r = lo + l.ry; r < hi; r += l.ny) {
             float f[V];
             PackedVec<T, V>::load(f, x + (int64_t)r * p.ldx + cv * V);
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = act_value<ACT, sizeof(T) == 4>(fmaf((f[i] - m[i]) * rs[i], w[i], b[i]));
+            for (int i = 0; i < V; ++i) f[i] = act_value<ACT, sizeof(T) == 4>(fmaf(centre<T>(f[i], m[i], ml[i]) * rs[i], w[i], b[i]));
             PackedVec<T, V>::store(y + (int64_t)r * p.C + cv * V, f);
         }
     }
@@ -241,17 +257,17 @@ __global__ __launch_bounds__(NTH) void gn_bwd_sums_kernel(const NormArgs p) {
     const Lanes l = lanes_of(p.C / V);
     const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row0 * p.ldx;
     const T* dy = reinterpret_cast<const T*>(p.dy) + (int64_t)tile.row0 * p.lddy;
-    const float *mean = p.mean + (int64_t)tile.doc * p.G, *rstd = p.rstd + (int64_t)tile.doc * p.G;
+    const float *mean = p.mean + (int64_t)tile.doc * p.G, *rstd = p.rstd + (int64_t)tile.doc * p.G, *rest = p.rest + (int64_t)tile.doc * p.G;
     float2* out = reinterpret_cast<float2*>(p.cpart) + ((int64_t)(p.base[tile.doc] + tile.i0 / PACKED_TILE) * p.sub + blockIdx.y) * p.C;
     const int cg = p.C / p.G;
     for (int c0 = 0; c0 < p.C / V; c0 += l.nx) {
         const int cv = c0 + l.cx;
         if (l.ry < l.ny && cv < p.C / V) {
-            float m[V], rs[V], w[V], b[V], s[V], q[V];
+            float m[V], rs[V], ml[V], w[V], b[V], s[V], q[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int c = cv * V + i, g = c / cg;
-                m[i] = mean[g]; rs[i] = rstd[g]; w[i] = p.w[c]; b[i] = p.b[c]; s[i] = 0.f; q[i] = 0.f;
+                m[i] = mean[g]; rs[i] = rstd[g]; ml[i] = rest[g]; w[i] = p.w[c]; b[i] = p.b[c]; s[i] = 0.f; q[i] = 0.f;
             }
 #pragma unroll 2
             for (int r = lo + l.ry; r < hi; r += l.ny) {
@@ -260,7 +276,7 @@ __global__ __launch_bounds__(NTH) void gn_bwd_sums_kernel(const NormArgs p) {
                 PackedVec<T, V>::load(d, dy + (int64_t)r * p.lddy + cv * V);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float hat = (f[i] - m[i]) * rs[i];
+                    const float hat = centre<T>(f[i], m[i], ml[i]) * rs[i];
                     const float dz = d[i] * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i]));
                     s[i] += dz;
                     q[i] = fmaf(dz, hat, q[i]);
@@ -355,15 +371,15 @@ __global__ __launch_bounds__(NTH) void gn_bwd_apply_kernel(const NormArgs p) {
     const Lanes l = lanes_of(p.C / V);
     const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row0 * p.ldx;
     const T* dy = reinterpret_cast<const T*>(p.dy) + (int64_t)tile.row0 * p.lddy;
-    const float *mean = p.mean + (int64_t)tile.doc * p.G, *rstd = p.rstd + (int64_t)tile.doc * p.G;
+    const float *mean = p.mean + (int64_t)tile.doc * p.G, *rstd = p.rstd + (int64_t)tile.doc * p.G, *rest = p.rest + (int64_t)tile.doc * p.G;
     const float2* coef = reinterpret_cast<const float2*>(p.coef) + (int64_t)tile.doc * p.G;
     const int cg = p.C / p.G;
     for (int cv = l.cx; cv < p.C / V && l.ry < l.ny; cv += l.nx) {
-        float m[V], rs[V], w[V], b[V], c1[V], c2[V];
+        float m[V], rs[V], ml[V], w[V], b[V], c1[V], c2[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = cv * V + i, g = c / cg;
-            m[i] = mean[g]; rs[i] = rstd[g]; w[i] = p.w[c]; b[i] = p.b[c];
+            m[i] = mean[g]; rs[i] = rstd[g]; ml[i] = rest[g]; w[i] = p.w[c]; b[i] = p.b[c];
             const float2 k = coef[g];
             c1[i] = k.x; c2[i] = k.y;
         }
@@ -374,7 +390,7 @@ __global__ __launch_bounds__(NTH) void gn_bwd_apply_kernel(const NormArgs p) {
             PackedVec<T, V>::load(d, dy + (int64_t)r * p.lddy + cv * V);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float hat = (f[i] - m[i]) * rs[i];
+                const float hat = centre<T>(f[i], m[i], ml[i]) * rs[i];
                 const float gw = d[i] * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i])) * w[i];
                 f[i] = rs[i] * (gw - c1[i] - hat * c2[i]);
             }
@@ -461,17 +477,18 @@ __global__ __launch_bounds__(RT, 4) void gn_resident_fwd_kernel(const NormArgs p
     const double2 t = group_sums<RT>(s, q, g, sl.gs, part);
     if (!on) return;
     const double count = (double)len * (double)cg, md = t.x / count, var = fmax(t.y / count - md * md, 0.0);
-    const float m = (float)md, rs = (float)(1.0 / sqrt(var + (double)p.eps));
+    const float m = (float)md, rs = (float)(1.0 / sqrt(var + (double)p.eps)), ml = (float)(md - (double)m);
     if (p.mean && ry == 0 && cx * V % cg == 0) {
         p.mean[(int64_t)doc * p.G + c0 / cg + g] = m;
         p.rstd[(int64_t)doc * p.G + c0 / cg + g] = rs;
+        p.rest[(int64_t)doc * p.G + c0 / cg + g] = ml;
     }
     float w[V], b[V];
     PackedVec<float, V>::load(w, p.w + c0 + cx * V);
     PackedVec<float, V>::load(b, p.b + c0 + cx * V);
     auto apply = [&](float (&f)[V], int r) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = act_value<ACT, sizeof(T) == 4>(fmaf((f[i] - m) * rs, w[i], b[i]));
+        for (int i = 0; i < V; ++i) f[i] = act_value<ACT, sizeof(T) == 4>(fmaf(centre<T>(f[i], m, ml) * rs, w[i], b[i]));
         PackedVec<T, V>::store(y + (int64_t)r * p.C, f);
     };
 #pragma unroll
@@ -520,12 +537,12 @@ __global__ __launch_bounds__(RT, 4) void gn_resident_bwd_kernel(const NormArgs p
     }
     const int g = on ? cx * V / cg : -1;
     const int64_t stat = (int64_t)doc * p.G + c0 / cg + max(g, 0);
-    const float m = p.mean[stat], rs = p.rstd[stat];
+    const float m = p.mean[stat], rs = p.rstd[stat], ml = p.rest[stat];
     float w[V], b[V], s[V], q[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) { const int c = c0 + min(cx, nx - 1) * V + i; w[i] = p.w[c]; b[i] = p.b[c]; s[i] = 0.f; q[i] = 0.f; }
     auto gather = [&](float xv, float dv, int i) {
-        const float hat = (xv - m) * rs, dz = dv * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i]));
+        const float hat = centre<T>(xv, m, ml) * rs, dz = dv * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i]));
         s[i] += dz;
         q[i] = fmaf(dz, hat, q[i]);
     };
@@ -576,7 +593,7 @@ __global__ __launch_bounds__(RT, 4) void gn_resident_bwd_kernel(const NormArgs p
     auto apply = [&](float (&f)[V], const float (&d)[V], int r) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float hat = (f[i] - m) * rs;
+            const float hat = centre<T>(f[i], m, ml) * rs;
             const float gw = d[i] * act_slope<ACT, sizeof(T) == 4>(fmaf(hat, w[i], b[i])) * w[i];
             f[i] = rs * (gw - c1 - hat * c2);
         }
@@ -665,7 +682,7 @@ void forward(NormArgs p, int act, int64_t longest, hipStream_t s) {
     const bool direct = cdiv(longest, PACKED_TILE) * p.sub * p.G <= 2048;
     if (!direct) hipLaunchKernelGGL(gn_finish_kernel, dim3((unsigned)p.B), dim3(NTH), 0, s, p);
 #define A(ACT_)                                                                                                                                 \
-    if (direct) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_, true>), grid, dim3(NTH), (unsigned)(2 * p.G * sizeof(float)), s, p);             \
+    if (direct) hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_, true>), grid, dim3(NTH), (unsigned)(3 * p.G * sizeof(float)), s, p);             \
     else hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT_, false>), grid, dim3(NTH), 0, s, p)
     if (act == ACT_RELU) { A(ACT_RELU); } else if (act == ACT_GELU) { A(ACT_GELU); } else if (act == ACT_SILU) { A(ACT_SILU); } else { A(ACT_NONE); }
 #undef A
@@ -702,7 +719,7 @@ extern "C" int osp_group_norm_fwd(const void* x, int64_t ldx, int64_t bf16, cons
     OSP_CHECK_ARG(B > 0 && M > 0 && longest > 0 && C > 0 && C <= MAXC && G > 0 && C % G == 0 && ldx >= C, "channels (at most 2048) must be a multiple of groups");
     OSP_CHECK_ARG(eps > 0.f && act >= ACT_NONE && act <= ACT_SILU && cap > 0 && cap < (int64_t)1 << 30 && packed_aligned(workspace, 16), "bad eps, activation or workspace");
     NormArgs p = {};
-    p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.out = y; p.mean = stats; p.rstd = stats + B * G; p.part = reinterpret_cast<double*>(workspace);
+    p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.out = y; p.mean = stats; p.rstd = stats + B * G; p.rest = stats + 2 * B * G; p.part = reinterpret_cast<double*>(workspace);
     p.begin = begin; p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
     p.B = (int)B; p.C = (int)C; p.G = (int)G; p.cap = (int)cap; p.sub = parts(M); p.eps = eps;
     const int V = bf16 ? 8 : 4;
@@ -722,7 +739,7 @@ extern "C" int osp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, i
     OSP_CHECK_ARG(act >= ACT_NONE && act <= ACT_SILU && cap > 0 && cap < (int64_t)1 << 30 && packed_aligned(workspace, 16), "bad activation or workspace");
     NormArgs p = {};
     p.x = x; p.ldx = ldx; p.dy = dy; p.lddy = lddy; p.w = w; p.b = b; p.out = dx;
-    p.mean = const_cast<float*>(stats); p.rstd = p.mean + B * G; p.dw = dw; p.db = db; p.add_w = (int)(add_w != 0); p.add_b = (int)(add_b != 0);
+    p.mean = const_cast<float*>(stats); p.rstd = p.mean + B * G; p.rest = p.mean + 2 * B * G; p.dw = dw; p.db = db; p.add_w = (int)(add_w != 0); p.add_b = (int)(add_b != 0);
     p.begin = begin; p.len = len; p.base = base; p.tiles = reinterpret_cast<const PackedTile*>(tiles); p.ntiles = ntiles;
     p.B = (int)B; p.C = (int)C; p.G = (int)G; p.cap = (int)cap; p.sub = parts(M);
     const int64_t slots = (M / PACKED_TILE + B) * p.sub;

@@ -212,11 +212,11 @@ def _workspace(nbytes, device):
 
 
 def _normalise(x, w, b, groups, rows, eps, act):
-    """-> (x as the kernel read it, y, mean and rstd)"""
+    """-> (x as the kernel read it, y, mean, rstd and the mean's part below 32 bits)"""
     x = _matrix(x, "x")
     M, C = x.shape
     y = torch.empty((M, C), device=x.device, dtype=x.dtype)
-    stats = torch.empty((2, rows.docs, groups), device=x.device, dtype=torch.float32)
+    stats = torch.empty((3, rows.docs, groups), device=x.device, dtype=torch.float32)
     if M:
         ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 0), x.device)
         call("osp_group_norm_fwd", x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, y, stats, ws, rows.begin, rows.length, rows.base, rows.tiles,

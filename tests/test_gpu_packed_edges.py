@@ -116,3 +116,46 @@ def test_queries_that_see_nothing_may_hold_nan(dtype, cap, slope, pairs, H, S, D
     for a, b in zip(*out):
         assert torch.isfinite(a).all() and torch.equal(a, b)
     assert float(out[1][0][blind].detach().abs().max()) == 0.0 and float(out[1][1][blind].abs().max()) == 0.0
+
+
+@gpu
+@pytest.mark.parametrize("lengths,C,G", [([300], 64, 4), ([90, 7], 30, 3), ([3000, 400], 64, 4), ([40], 2048, 32)])
+def test_group_norm_resolves_values_far_from_zero(lengths, C, G):
+    """f32 x = 4096 + noise of 0.1, values taken as given: the mean is kept with more than 32 bits, so xhat is not shifted by its rounding (u 4096 / 0.1 =
+    2.4e-3).  What remains: sums in 64 bits (at most 512 additions in one chain, each 2^-53 of a sum whose squares are (mean / deviation)^2 times the
+    variance) make rstd uncertain by r = 256 2^-53 (mean / deviation)^2, and 3 u for the difference, its product and rstd's rounding: e = r + 3 u relative
+    to xhat, and for the mean 512 2^-53 |mean| rstd.  Gradients (act None: dz = dy): chains of at most 128 rows in 32 bits as in the other group norm tests,
+    140 u of the sums of absolute values."""
+    from optispeech_amd import packed_ops as P
+    M = sum(lengths)
+    x, g = randn(M, C, seed=21, std=0.1) + 4096.0, randn(M, C, seed=22)
+    w, b = torch.nn.Parameter(randn(C, seed=23) * 0.2 + 1), torch.nn.Parameter(randn(C, seed=24))
+    xr = x.clone().requires_grad_()
+    rows = P.PackedRows.from_offsets(offsets(lengths), M)
+    y = P.group_norm(xr, w, b, G, rows, 1e-8)
+    (dx,) = torch.autograd.grad(y, (xr,), g)
+    docs = ref.documents(lengths)
+    X, W, B = (t.detach().double().cpu().requires_grad_() for t in (x, w, b))
+    want = ref.group_norm(X, W, B, docs, G, 1e-8, None)
+    wx, ww, wb = torch.autograd.grad(want, (X, W, B), g.double().cpu())
+    X, W, B, g = X.detach(), W.detach(), B.detach(), g.double().cpu()
+    ytol, xtol, wtol, btol = torch.zeros_like(X), torch.zeros_like(X), torch.zeros(C).double(), torch.zeros(C).double()
+    for sl in docs:
+        n = sl.stop - sl.start
+        xg = X[sl].reshape(n, G, C // G)
+        m = xg.mean((0, 2), keepdim=True)
+        var = ((xg - m) ** 2).mean((0, 2), keepdim=True)
+        full = lambda t: t.expand(n, G, C // G).reshape(n, C)                                     # noqa: E731
+        mean = lambda t: full(t.reshape(n, G, C // G).mean((0, 2), keepdim=True))                # noqa: E731
+        rs = full(1 / torch.sqrt(var + 1e-8))
+        hat = full((xg - m)) * rs
+        e = (full(256 * 2.0 ** -53 * m * m / var) + 3 * U) * hat.abs() + 512 * 2.0 ** -53 * full(m.abs()) * rs
+        ytol[sl] = e * W.abs() + 3 * U * ((hat * W).abs() + B.abs())
+        gw = (g[sl] * W).abs()
+        m2 = mean(gw * hat.abs())
+        xtol[sl] = rs * (150 * U * (gw + mean(gw) + hat.abs() * m2) + e * m2 + hat.abs() * mean(gw * e)) + (256 * 2.0 ** -53 * full(m * m / var)) * wx[sl].abs()
+        wtol += (g[sl].abs() * (e + 140 * U * hat.abs())).sum(0)
+        btol += 140 * U * g[sl].abs().sum(0)
+    for name, a, t, tol in (("y", y, want, ytol), ("dx", dx, wx, xtol), ("dw", w.grad, ww, wtol), ("db", b.grad, wb, btol)):
+        err = (a.detach().double().cpu() - t.detach()).abs()
+        assert bool((err <= tol + U * t.detach().abs()).all()), (name, (err - tol).max().item(), err.max().item())

@@ -143,7 +143,8 @@ REPLACES = {
                   "relative positions: generator/modules/_transformer/embedding.py:91-124,252-322)",
     "osp_group_norm_workspace_bytes": "workspace query for osp_group_norm_fwd / osp_group_norm_bwd",
     "osp_group_norm_fwd": "no reference counterpart: group norm + activation over the rows of each document (the place of BatchNorm + swish in "
-                          "_conformer/convolution.py:61-70, which counts padded frames)",
+                          "_conformer/convolution.py:61-70, which counts padded frames); stats: (3, B, G) f32, mean, 1 / deviation and the mean's "
+                          "part below f32",
     "osp_group_norm_bwd": "autograd of the same",
     "osp_packed_attention_fwd": "MultiHeadedAttention.forward_attention on packed documents, with capped scores, a penalty on distance, causal and prefix "
                                 "masks, shared key heads and different query / key counts (generator/modules/_transformer/attention.py:75-125 "
