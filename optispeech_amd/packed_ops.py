@@ -236,23 +236,26 @@ def _grad_target(p):
 
 class GroupNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, anchor, params, groups, rows, eps, act):
-        w, b = params
+    def forward(ctx, x, anchor, wc, bc, params, groups, rows, eps, act):
+        """wc, bc: a weight or bias that was computed (its gradient goes back to what it was computed from); params: those that are leaves"""
+        w, b = params[0] if wc is None else wc, params[1] if bc is None else bc
         x, y, stats = _normalise(x, w, b, groups, rows, eps, act)
-        ctx.save_for_backward(x, stats)
+        ctx.save_for_backward(x, stats, wc, bc)
         ctx.params, ctx.cfg = params, (groups, rows, act)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         _first_order()
-        x, stats = ctx.saved_tensors
+        x, stats, wc, bc = ctx.saved_tensors
         (w, b), (groups, rows, act) = ctx.params, ctx.cfg
         M, C = x.shape
         dy = _matrix(dy, "dy")
         dx = torch.empty((M, C), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
-        db, add_b = _grad_target(b)                                # the kernels write db first, then dw: one tensor may be both
-        dw, add_w = _grad_target(w)
+        # (the kernels write db first, then dw: one tensor may be both)
+        db, add_b = _grad_target(b) if bc is None else (torch.empty_like(bc), 0)
+        dw, add_w = _grad_target(w) if wc is None else (torch.empty_like(wc), 0)
+        w, b = w if wc is None else wc, b if bc is None else bc
         if M:
             ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 1), x.device)
             call("osp_group_norm_bwd", dy, dy.stride(0), x, x.stride(0), int(x.dtype == torch.bfloat16), w, b, stats, dx, dw, add_w, db, add_b, ws,
@@ -261,12 +264,13 @@ class GroupNormFn(torch.autograd.Function):
             for t, add in ((dx, 0), (dw, add_w), (db, add_b)):
                 if t is not None and not add:
                     t.zero_()
-        return dx, None, None, None, None, None, None
+        return dx, None, None if wc is None else dw, None if bc is None else db, None, None, None, None, None
 
 
 def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
     """act(weight * (x - mean) / sqrt(var + eps) + bias), mean and variance over a document's rows and a group's channels.  x (M, C) float32
-    or bfloat16 (any row stride), weight / bias (C,) float32, act None, "relu", "gelu" (with erf) or "silu"; C <= 2048."""
+    or bfloat16 (any row stride), weight / bias (C,) float32, act None, "relu", "gelu" (with erf) or "silu"; C <= 2048.  The gradients of weights that are
+    leaves are added to their ``.grad``; those of computed weights (1 + gamma) go through autograd."""
     if x.dim() != 2 or not x.is_cuda:
         raise OspError("x must be a (rows, channels) tensor on the GPU")
     if x.dtype not in (torch.float32, torch.bfloat16):
@@ -285,9 +289,11 @@ def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
     if not _wants_grad(x, weight, bias):
         return _normalise(x, weight, bias, int(groups), rows, float(eps), ACTS[act])[1]
     # The parameters stay out of the autograd graph (the kernels write their gradients), so a captured backward meets no node of an eager graph;
-    # where x has no gradient a leaf of the call's own keeps the backward reachable.
-    anchor = None if x.requires_grad else x.new_empty(0, dtype=torch.float32).requires_grad_()
-    return GroupNormFn.apply(x, anchor, (weight, bias), int(groups), rows, float(eps), ACTS[act])
+    # where nothing else has a gradient a leaf of the call's own keeps the backward reachable.
+    wc, bc = (t if t.requires_grad and not t.is_leaf else None for t in (weight, bias))
+    anchor = None if x.requires_grad or wc is not None or bc is not None else x.new_empty(0, dtype=torch.float32).requires_grad_()
+    params = (weight if wc is None else None, bias if bc is None else None)
+    return GroupNormFn.apply(x, anchor, wc, bc, params, int(groups), rows, float(eps), ACTS[act])
 
 
 # ------------------------------------------------------------------------------------------------------------------ attention over documents

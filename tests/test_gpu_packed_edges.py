@@ -159,3 +159,42 @@ def test_group_norm_resolves_values_far_from_zero(lengths, C, G):
     for name, a, t, tol in (("y", y, want, ytol), ("dx", dx, wx, xtol), ("dw", w.grad, ww, wtol), ("db", b.grad, wb, btol)):
         err = (a.detach().double().cpu() - t.detach()).abs()
         assert bool((err <= tol + U * t.detach().abs()).all()), (name, (err - tol).max().item(), err.max().item())
+
+
+@gpu
+@pytest.mark.parametrize("needs_x", [True, False])
+@pytest.mark.parametrize("lengths,C", [([50, 31], 32), ([50, 31], 10), ([1500], 512)])
+def test_group_norm_weights_computed_from_parameters(needs_x, lengths, C):
+    """a weight or bias that is itself a result (1 + gamma, a scaled table) hands its gradient on: bit for bit what a parameter of its value is given, and
+    nothing is written beside it"""
+    from optispeech_amd import packed_ops as P
+    M = sum(lengths)
+    rows = P.PackedRows.from_offsets(offsets(lengths), M)
+    x, g = randn(M, C, seed=1).requires_grad_(needs_x), randn(M, C, seed=2)
+    gamma, beta = torch.nn.Parameter(randn(C, seed=3)), torch.nn.Parameter(randn(C, seed=4))
+    w, b = torch.nn.Parameter(1 + gamma.detach()), torch.nn.Parameter(beta.detach() * 2)
+    y0 = P.group_norm(x, w, b, 2, rows, act="silu")
+    y0.backward(g)
+    for wt, bt in ((1 + gamma, beta * 2), (1 + gamma, b), (w, beta * 2)):
+        for p in (gamma, beta, w, b, x):
+            if p is not w and p is not b:
+                p.grad = None
+        dw, db = w.grad.clone(), b.grad.clone()
+        w.grad = b.grad = None
+        y = P.group_norm(x, wt, bt, 2, rows, act="silu")
+        assert torch.equal(y, y0)
+        y.backward(g)
+        assert torch.equal(gamma.grad if wt is not w else w.grad, dw)
+        assert torch.equal(beta.grad / 2 if bt is not b else b.grad, db)
+        w.grad, b.grad = dw, db
+    both = 1 + gamma                                                # one result as weight and bias: autograd adds the two gradients
+    gamma.grad = w.grad = b.grad = None
+    P.group_norm(x, both, both, 2, rows, act="silu").backward(g)
+    one, two = torch.nn.Parameter(both.detach().clone()), torch.nn.Parameter(both.detach().clone())
+    P.group_norm(x, one, two, 2, rows, act="silu").backward(g)
+    assert torch.equal(gamma.grad, one.grad + two.grad)
+    y = P.group_norm(x, both, one, 2, rows)
+    with torch.no_grad():
+        both += 1                                                    # a kept result changed in place
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward(g)
