@@ -225,13 +225,14 @@ def _normalise(x, w, b, groups, rows, eps, act):
 
 
 def _grad_target(p):
-    """(param.grad, 1 where the kernel adds to it, 0 where it was made just now and is written)"""
+    """(tensor the kernel writes, 1 where it adds to what is there): param.grad, made here where there is none, or a tensor of its own beside a strided one
+    (the kernels take contiguous channels), which the caller adds"""
     if not _want(p):
         return None, 0
     if p.grad is None:
         p.grad = torch.empty_like(p)
         return p.grad, 0
-    return p.grad, 1
+    return (p.grad, 1) if p.grad.is_contiguous() else (torch.empty_like(p), 0)
 
 
 class GroupNormFn(torch.autograd.Function):
@@ -255,6 +256,7 @@ class GroupNormFn(torch.autograd.Function):
         # (the kernels write db first, then dw: one tensor may be both)
         db, add_b = _grad_target(b) if bc is None else (torch.empty_like(bc), 0)
         dw, add_w = _grad_target(w) if wc is None else (torch.empty_like(wc), 0)
+        strided = [(p, g) for p, g in ((b, db), (w, dw)) if _want(p) and not p.grad.is_contiguous()]
         w, b = w if wc is None else wc, b if bc is None else bc
         if M:
             ws = _workspace(_size("osp_group_norm_workspace_bytes", rows.docs, M, C, groups, 1), x.device)
@@ -264,6 +266,8 @@ class GroupNormFn(torch.autograd.Function):
             for t, add in ((dx, 0), (dw, add_w), (db, add_b)):
                 if t is not None and not add:
                     t.zero_()
+        for p, g in strided:
+            p.grad.add_(g)
         return dx, None, None if wc is None else dw, None if bc is None else db, None, None, None, None, None
 
 

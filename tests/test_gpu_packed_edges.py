@@ -198,3 +198,25 @@ def test_group_norm_weights_computed_from_parameters(needs_x, lengths, C):
         both += 1                                                    # a kept result changed in place
     with pytest.raises(RuntimeError, match="inplace"):
         y.backward(g)
+
+
+@gpu
+def test_group_norm_adds_to_strided_gradients():
+    """param.grad as every second element of a buffer: its elements receive the gradient, their neighbours stay"""
+    from optispeech_amd import packed_ops as P
+    lengths, C = [50, 31], 32
+    M = sum(lengths)
+    rows = P.PackedRows.from_offsets(offsets(lengths), M)
+    x, g = randn(M, C, seed=1).requires_grad_(), randn(M, C, seed=2)
+    w, b, p, s = (torch.nn.Parameter(randn(C, seed=3)) for _ in range(4))
+    bufs = [randn(2 * C, seed=5 + i) for i in range(3)]
+    kept = [t.clone() for t in bufs]
+    P.group_norm(x, w, b, 2, rows).backward(g)
+    dw, db = w.grad.clone(), b.grad.clone()
+    w.grad, b.grad, s.grad = (t[::2] for t in bufs)
+    P.group_norm(x, w, b, 2, rows).backward(g)
+    assert torch.equal(bufs[0][::2], kept[0][::2] + dw) and torch.equal(bufs[1][::2], kept[1][::2] + db)
+    P.group_norm(x, s, s, 2, rows).backward(g)
+    assert torch.equal(bufs[2][::2], kept[2][::2] + db + dw)
+    for t, k in zip(bufs, kept):
+        assert torch.equal(t[1::2], k[1::2])
