@@ -17,6 +17,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import precision as _precision
@@ -42,6 +43,15 @@ def _wants_grad(*ts):
 def _first_order():
     if torch.is_grad_enabled():                                   # create_graph: the gradients below would enter the graph as constants
         raise OspError("the packed operators have no second derivatives (create_graph=True)")
+
+
+def _no_tangents(*ts):
+    """a dual tensor has requires_grad false and an ordinary address: it would be taken as a constant"""
+    if forward_ad._current_level < 0:                             # (outside of every dual level there is none)
+        return
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise OspError("the packed operators have no forward-mode derivatives")
 
 
 class PackedRows:
@@ -176,6 +186,7 @@ def rotary(q, k, rope, rows, first=None, out_dtype=None):
     """Turn the first ``rope.channels`` channels of every head of q (M, heads, width) and k (M, shared, width) by the row's position: its index in
     its document plus ``first`` (docs,) int64 (the frames already in a cache).  One launch; results are contiguous, in ``out_dtype`` (float32
     or bfloat16; the inputs' type without it).  The gradient is the inverse turn, in the inputs' type."""
+    _no_tangents(q, k)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] < 1 or k.shape[1] < 1:
         raise OspError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must be (rows, heads, width) with the same rows and width")
     if q.dtype != k.dtype:
@@ -275,6 +286,7 @@ def group_norm(x, weight, bias, groups, rows, eps=1e-5, act=None):
     """act(weight * (x - mean) / sqrt(var + eps) + bias), mean and variance over a document's rows and a group's channels.  x (M, C) float32
     or bfloat16 (any row stride), weight / bias (C,) float32, act None, "relu", "gelu" (with erf) or "silu"; C <= 2048.  The gradients of weights that are
     leaves are added to their ``.grad``; those of computed weights (1 + gamma) go through autograd."""
+    _no_tangents(x, weight, bias)
     if x.dim() != 2 or not x.is_cuda:
         raise OspError("x must be a (rows, channels) tensor on the GPU")
     if x.dtype not in (torch.float32, torch.bfloat16):
@@ -379,6 +391,7 @@ def attention(q, k, v, rows, keys=None, causal=False, prefix=None, softcap=0.0, 
 
     float32 tensors are computed in exact 32-bit products, unless the package runs in its bf16 mode: then the operands are rounded to bf16, as in
     its other attention paths, and the result is float32.  Gradients for q, k and v; no attention dropout."""
+    _no_tangents(q, k, v, slopes)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise OspError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} must be (rows, heads, width), k and v alike")
     H, S, D = q.shape[1], k.shape[1], q.shape[2]

@@ -220,3 +220,25 @@ def test_group_norm_adds_to_strided_gradients():
     assert torch.equal(bufs[2][::2], kept[2][::2] + db + dw)
     for t, k in zip(bufs, kept):
         assert torch.equal(t[1::2], k[1::2])
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_derivatives_are_refused(dev):
+    """a dual tensor is not taken as a constant, in whichever place it stands"""
+    import torch.autograd.forward_ad as fwd
+    from optispeech_amd import packed_ops as P
+    from optispeech_amd._lib import OspError
+    rows = P.PackedRows.from_offsets(offsets([4]), 4) if dev == "cuda" else None
+    rope = P.Rotary(8, device=dev)
+    h, x, c = torch.randn(4, 2, 8, device=dev), torch.randn(4, 8, device=dev), torch.ones(8, device=dev)
+    s = torch.ones(2, device=dev)
+    with fwd.dual_level():
+        hd, xd, cd, sd = (fwd.make_dual(t, torch.ones_like(t)) for t in (h, x, c, s))
+        for f, args in ((P.rotary, (hd, h, rope, rows)), (P.rotary, (h, hd, rope, rows)), (P.group_norm, (xd, c, c, 2, rows)), (P.group_norm, (x, cd, c, 2, rows)),
+                        (P.group_norm, (x, c, cd, 2, rows)), (P.attention, (hd, h, h, rows)), (P.attention, (h, hd, h, rows)), (P.attention, (h, h, hd, rows))):
+            with pytest.raises(OspError, match="forward-mode"):
+                f(*args)
+        with pytest.raises(OspError, match="forward-mode"):
+            P.attention(h, h, h, rows, slopes=sd)
+        if dev == "cuda":                                            # plain tensors inside the level are computed as outside
+            assert torch.isfinite(P.attention(h, h, h, rows)).all()
