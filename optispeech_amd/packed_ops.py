@@ -141,6 +141,12 @@ class Rotary:
         self.turns = torch.tensor([x / (2.0 * math.pi) for x in f], dtype=torch.float64, device=device)
 
 
+def _copy(t):
+    """a dense copy on memory of its own.  (`contiguous()` hands back a contiguous tensor as it is: off 16 bytes in a larger buffer, or with a dimension of one
+    element whose stride says nothing)"""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _heads(t, name):
     """(M, heads, width) with contiguous channels; any row and head stride."""
     if t.dim() != 3:
@@ -149,7 +155,7 @@ def _heads(t, name):
         raise OspError(f"{name}: float32 or bfloat16, not {t.dtype}")
     if not t.is_cuda:
         raise OspError(f"{name} must live on the GPU")
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else _copy(t)
 
 
 def _rotate(q, k, rope, rows, first, out_dtype, inverse):
@@ -214,7 +220,7 @@ def _matrix(t, name):
         raise OspError(f"{name} must be (rows, channels), not {tuple(t.shape)}")
     if t.dtype not in (torch.float32, torch.bfloat16):
         raise OspError(f"{name}: float32 or bfloat16, not {t.dtype}")
-    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else _copy(t)
 
 
 def _workspace(nbytes, device):
@@ -318,7 +324,7 @@ def _aligned(t, name):
     t = _heads(t, name)
     e = 16 // t.element_size()
     r, h = t.stride(0), t.stride(1)
-    return t if r % e == 0 and h % e == 0 and t.data_ptr() % 16 == 0 and t.shape[2] <= r < 1 << 22 else t.contiguous()
+    return t if r % e == 0 and h % e == 0 and t.data_ptr() % 16 == 0 and t.shape[2] <= r < 1 << 22 else _copy(t)
 
 
 def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):

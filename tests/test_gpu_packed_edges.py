@@ -242,3 +242,71 @@ def test_forward_mode_derivatives_are_refused(dev):
             P.attention(h, h, h, rows, slopes=sd)
         if dev == "cuda":                                            # plain tensors inside the level are computed as outside
             assert torch.isfinite(P.attention(h, h, h, rows)).all()
+
+
+def _shifted(t):
+    """the same values, contiguous, one element behind a 16-byte border"""
+    return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [[70, 33], [1]])
+def test_contiguous_tensors_at_odd_addresses(dtype, lengths):
+    """contiguous inputs and gradients that do not start on 16 bytes, tables of one row: results of the aligned tensors, bit for bit"""
+    from optispeech_amd import packed_ops as P
+    H, D = 2, 32
+    M = sum(lengths)
+    rows = P.PackedRows.from_offsets(offsets(lengths), M)
+    t = [randn(M, H, D, seed=i, dtype=dtype) for i in range(4)]
+    odd = [_shifted(x) for x in t]
+    assert all(x.is_contiguous() and x.data_ptr() % 16 for x in odd)
+    want = grads(*t, rows, causal=True)
+    for args in (odd, odd[:3] + t[3:], t[:3] + odd[3:]):
+        for a, b in zip(grads(*args, rows, causal=True), want):
+            assert torch.equal(a, b)
+    with torch.no_grad():
+        for n in (M, 1):
+            r = P.PackedRows.from_offsets(offsets([n]), n, longest=n)
+            assert torch.equal(P.attention(odd[0][:n], odd[1], odd[2], r, keys=P.PackedRows.from_offsets(offsets([M]), M)),
+                               P.attention(t[0][:n], t[1], t[2], r, keys=P.PackedRows.from_offsets(offsets([M]), M)))
+        rope = P.Rotary(D)
+        for a, b in zip(P.rotary(odd[0], odd[1], rope, rows), P.rotary(t[0], t[1], rope, rows)):
+            assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_row_and_one_head_of_any_stride(dtype):
+    """dimensions of one element carry strides that say nothing; a projection's slice of one row, shifted by one element"""
+    from optispeech_amd import packed_ops as P
+    D = 16
+    rows = P.PackedRows.from_offsets(offsets([1]), 1)
+    flat = randn(3 * D + 1, seed=1, dtype=dtype)
+    views = [flat.as_strided((1, 1, D), s, o) for s in ((1, 1, 1), (3, 5, 1), (D, D, 1)) for o in (0, 1)]
+    for v in views:
+        c = v.clone(memory_format=torch.contiguous_format)
+        for a, b in zip(grads(v, v, v, v, rows), grads(c, c, c, c, rows)):
+            assert torch.equal(a, b)
+    w = randn(1, 3 * 2 * D + 1, seed=2, dtype=dtype)[:, 1:]
+    q, k, v = (w[:, i * 2 * D:(i + 1) * 2 * D].unflatten(1, (2, D)) for i in range(3))
+    for a, b in zip(grads(q, k, v, q, rows), grads(q.clone(), k.clone(), v.clone(), q.clone(), rows)):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_group_norm_of_one_row_of_any_stride(dtype):
+    from optispeech_amd import packed_ops as P
+    C = 24
+    rows = P.PackedRows.from_offsets(offsets([1]), 1)
+    w, b = randn(C, seed=3), randn(C, seed=4)
+    x, g = randn(C, 1, seed=1, dtype=dtype).t(), randn(C, 1, seed=2, dtype=dtype).t()
+    assert x.stride() == (1, 1)
+    out = []
+    for copy in (False, True):
+        xr, gr = ((t.clone(memory_format=torch.contiguous_format) if copy else t.detach()) for t in (x, g))
+        xr.requires_grad_()
+        y = P.group_norm(xr, w, b, 3, rows, act="silu")
+        out.append((y.detach(),) + torch.autograd.grad(y, (xr,), gr))
+    assert all(torch.equal(p, q) for p, q in zip(*out))
