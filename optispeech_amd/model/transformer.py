@@ -142,8 +142,8 @@ class Encoder(nn.Module):
         super().__init__()
         if packed is None or packed.get("rotary") is None:
             self.embed = nn.Sequential(ScaledPositionalEncoding(attention_dim, positional_dropout_rate))
-        else:                                                     # positions enter with the queries and keys
-            self.embed = None
+        else:                                                     # positions enter with the queries and keys; the dropout stays
+            self.embed, self.pos_drop, self._s = None, positional_dropout_rate, rng.new_stream()
 
         def attention():
             if packed is None:
@@ -157,8 +157,7 @@ class Encoder(nn.Module):
 
     def forward(self, xs, klen):
         """klen: the valid-key counts, or the PackedRows of the frames where the attention is the packed one"""
-        if self.embed is not None:
-            xs = self.embed(xs)
+        xs = self.embed(xs) if self.embed is not None else _dropout(xs, self.pos_drop, self.training, self._s)
         for layer in self.encoders:
             xs = layer(xs, klen)
         return self.after_norm(xs)

@@ -310,3 +310,25 @@ def test_group_norm_of_one_row_of_any_stride(dtype):
         y = P.group_norm(xr, w, b, 3, rows, act="silu")
         out.append((y.detach(),) + torch.autograd.grad(y, (xr,), gr))
     assert all(torch.equal(p, q) for p, q in zip(*out))
+
+
+@gpu
+def test_rotary_transformer_keeps_its_positional_dropout():
+    """positional_dropout_rate acts on the frames that enter the first layer, in training only"""
+    from optispeech_amd import rng
+    from optispeech_amd.model.transformer import Transformer
+    x, pad = randn(2, 40, 64, seed=1), torch.zeros(2, 40, dtype=torch.bool, device=DEV)
+    out = {}
+    for rate in (0.0, 0.5):
+        torch.manual_seed(3)
+        m = Transformer(dim=64, attention_heads=4, linear_units=96, num_blocks=0, dropout_rate=0.0, positional_dropout_rate=rate, attention_dropout_rate=0.0,
+                        selfattention_layer_type="packed", packed=dict(rotary={})).to(DEV)
+        for training in (False, True):
+            rng.manual_seed(11, 0)
+            with torch.no_grad():
+                out[rate, training] = m.train(training)(x, pad)
+    assert torch.equal(out[0.0, True], out[0.0, False]) and torch.equal(out[0.5, False], out[0.0, False])
+    # no blocks: the final norm of the dropped frames.  Dropped channels share one value per row (before weight and bias): about half of them
+    y = out[0.5, True]
+    low = (y - y.median(-1, keepdim=True).values).abs() < 1e-6
+    assert not torch.equal(y, out[0.0, True]) and 0.4 < low.float().mean().item() < 0.6
