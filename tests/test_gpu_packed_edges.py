@@ -332,3 +332,50 @@ def test_rotary_transformer_keeps_its_positional_dropout():
     y = out[0.5, True]
     low = (y - y.median(-1, keepdim=True).values).abs() < 1e-6
     assert not torch.equal(y, out[0.0, True]) and 0.4 < low.float().mean().item() < 0.6
+
+
+@gpu
+def test_taped_segments_with_the_packed_attention_equal_eager():
+    """The Transformer backbone with packed attention, f32: the recorded acoustic model replayed on ANOTHER ragged batch of the same padded shape (other lengths, so
+    other documents).  Steps: batch 0 twice (the second records), 1, 1, 0 without an optimizer update; gradients of both networks, taped against
+    eager, to the tolerance of two eager runs (f32 atomics of the weight-gradient kernels)."""
+    from oracle import schema as S
+    from optispeech_amd import precision, rng, tape
+    from optispeech_amd.config import ModelConfig, make_optispeech, synthetic_batch
+    precision.set_precision("f32")
+    keep = tape.ENABLED
+
+    def run(tapes):
+        tape.ENABLED = tapes
+        c = S.SMALL
+        cfg = ModelConfig(dim=c.dim, enc_inter=c.enc_inter, dec_inter=c.dec_inter, dur=c.dur + (0.0,), pitch=c.pitch + (0.0,),
+                          energy=c.energy + (0.0,), voc_dim=c.voc_dim, voc_inter=c.voc_inter, voc_layers=c.voc_layers,
+                          backbone="transformer", packed_attention=dict(rotary={}, softcap=30.0, distance_slopes=True)).no_dropout()
+        torch.manual_seed(7)
+        rng.manual_seed(7, 0)
+        m = make_optispeech(cfg, batch_size=2, pretraining_steps=0).to(DEV).train()
+        m.tape_segments = True
+        got = {}
+        for name, o in zip(("g", "d"), m.optimizers()):
+            o.step = (lambda n, oo: (lambda *a, **k: got.__setitem__(n, oo.arena.grad.detach().clone())))(name, o)
+        out = []
+        for r in (0, 0, 1, 1, 0):
+            b = synthetic_batch(2, 24, 96, cfg, seed=50 + r, ragged=True, device=DEV)
+            m.generator.segment_rand01 = torch.tensor([0.25 + 0.5 * r, 0.6 - 0.3 * r], device=DEV)
+            m.training_step(b, 0)
+            torch.cuda.synchronize()
+            out.append((got["g"].clone(), got["d"].clone()))
+        names = [r[0].meta["names"] for r in m._tape_am.cache.values() if r is not tape.EAGER] if tapes else []
+        return out, names
+
+    try:
+        s0 = tape.stats()
+        (a, _), (b, names) = run(False), run(True)
+        s1 = tape.stats()
+    finally:
+        tape.ENABLED = keep
+    assert s1["replayed"] - s0["replayed"] >= 6 and s1["poisoned"] == s0["poisoned"], (s0, s1)
+    assert names and any("osp_packed_attention_fwd" in n for n in names)
+    for i, ((ga, da), (gb, db)) in enumerate(zip(a, b)):
+        assert ((ga - gb).norm() / ga.norm()).item() < 1e-5, (i, "generator")
+        assert ((da - db).norm() / da.norm()).item() < 1e-5, (i, "discriminator")
