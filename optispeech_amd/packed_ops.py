@@ -335,12 +335,14 @@ def _attend(q, k, v, rows, keys, causal, prefix, softcap, slopes, scale, save):
     lse = torch.empty((H, M), device=q.device, dtype=torch.float32) if save else None
     rest = torch.empty_like(o) if save and bf16 else None
     # new tokens over a cache: the queries that share a key head fit the 32 columns of one score tile (csrc/attention_packed_token.hip).  Its workspace
-    # holds every row of the table per split, at most 34 MB where the rows are the documents'; a far larger table takes the other form.
-    few = M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536
+    # holds every row of the table per split: where the rows are the documents', at most 128 (width + 2) bytes x (2048 + documents x key heads).  It may take as
+    # much memory as the keys and values that the call reads, or 256 MB; a table whose rows outgrow both takes the other form (8192 documents of 512 keys, 64 / 8
+    # heads of 128, 260 MB beside 17 GB: 3.9 and 18.3 ms).
+    few = M and not save and rows.longest * (H // S) <= 32 and keys.longest and rows.docs < 65536 and H < 65536
     nbytes = _size("osp_packed_attention_token_workspace_bytes", rows.docs, M, keys.longest, H, S, D) if few else 0
     if not k.shape[0]:                                            # no keys at all: nothing is seen
         o.zero_()
-    elif few and nbytes <= 1 << 28:
+    elif few and nbytes <= max(1 << 28, 2 * k.numel() * k.element_size()):
         ws = _workspace(nbytes, q.device)
         call("osp_packed_attention_token", q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), bf16, o, ws,
              rows.begin, rows.length, rows.tiles, rows.ntiles, rows.cap, keys.begin, keys.length, keys.longest, prefix, slopes, rows.docs, M, H, S,

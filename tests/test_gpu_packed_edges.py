@@ -379,3 +379,27 @@ def test_taped_segments_with_the_packed_attention_equal_eager():
     for i, ((ga, da), (gb, db)) in enumerate(zip(a, b)):
         assert ((ga - gb).norm() / ga.norm()).item() < 1e-5, (i, "generator")
         assert ((da - db).norm() / da.norm()).item() < 1e-5, (i, "discriminator")
+
+
+@gpu
+def test_new_tokens_for_many_documents(monkeypatch):
+    """40 000 documents: the split kernel's workspace passes 256 MB but not the cache, and the call stays with it; documents all over the batch against the
+    definition, rows of no document zero"""
+    from optispeech_amd import packed_ops as P
+    B, T, H, S, D = 40000, 64, 32, 4, 64
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q = torch.randn(B + 3, H, D, generator=g, device=DEV).bfloat16()
+    k, v = (torch.randn(B * T, S, D, generator=g, device=DEV).bfloat16() for _ in range(2))
+    klens = torch.arange(B, device=DEV) % (T + 1)
+    rows = P.PackedRows.from_offsets(torch.arange(B + 1, device=DEV), B + 3, longest=1)
+    names, call = [], P.call
+    monkeypatch.setattr(P, "call", lambda name, *a: (names.append(name), call(name, *a)))
+    o = P.attention(q, k, v, rows, keys=P.PackedRows.from_padded(klens, T), causal=True)
+    assert "osp_packed_attention_token" in names
+    assert P._size("osp_packed_attention_token_workspace_bytes", B, B + 3, T, H, S, D) > 1 << 28
+    for b in (0, 1, 63, 64, 65, 20001, 33333, B - 1):
+        n = int(klens[b])
+        want, tol = bounds(q[b:b + 1], k[b * T:b * T + n], v[b * T:b * T + n], q[b:b + 1], [slice(0, 1)], [slice(0, n)], D ** -0.5, True, None, 0.0, None,
+                           torch.bfloat16)
+        close((o[b:b + 1],), want[:1], tol[:1])
+    assert float(o[B:].abs().max()) == 0.0
