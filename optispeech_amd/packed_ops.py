@@ -391,7 +391,7 @@ def attention(q, k, v, rows, keys=None, causal=False, prefix=None, softcap=0.0, 
     ``rows`` (PackedRows) lays out the queries; ``keys`` the keys where they differ (a cache: ``PackedRows.from_padded(lengths, capacity)``), with the
     same number of documents.  Query i of a document stands at position  keys - queries + i : the last query is at the last key.
 
-    score = c(scale q . k) - slopes[head] |position - j|, with c(x) = softcap tanh(x / softcap) where softcap > 0 (and softcap / scale between 1e-30 and 1e30);
+    score = c(scale q . k) - slopes[head] |position - j|, with c(x) = softcap tanh(x / softcap) where softcap > 0 (it and scale / softcap between 1e-36 and 1e36);
     scale (positive) 1 / sqrt(width) unless given;
     slopes (heads,) float32 (no gradient).  ``causal``: key j is seen from position j on; ``prefix`` (docs,) int64 with it: the first prefix keys of
     a document are seen by all its queries.  A query that sees nothing gives zeros, and so do rows of no document; gradients likewise.
@@ -418,8 +418,8 @@ def attention(q, k, v, rows, keys=None, causal=False, prefix=None, softcap=0.0, 
     scale = D ** -0.5 if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise OspError(f"scale {scale}: positive")
-    if softcap and not 1e-30 <= scale / softcap <= 1e30:
-        raise OspError(f"softcap {softcap} is out of range for the scale {scale}: their quotient must lie between 1e-30 and 1e30")
+    if softcap and not (1e-36 <= softcap <= 1e36 and 1e-36 <= scale / softcap <= 1e36):
+        raise OspError(f"softcap {softcap} with scale {scale}: the cap and their quotient must lie between 1e-36 and 1e36")
     keys = rows if keys is None else keys
     rows._check(q, "q")
     keys._check(k, "k")
