@@ -8,8 +8,8 @@
 // S and dP are computed twice, 7 instead of 5 products per tile pair: the price of combining dQ without atomics or a partial dQ per key tile.
 // dK / dV keeps V's 128 rows in LDS: with K's and V's fragments both in registers a SIMD held one wave (6.67 ms, below 3.09 ms).
 //
-// Measured (bf16, 16 heads of 128 sharing 4, capped scores, 5 documents of 1000 .. 8192 rows under a prefix mask): dQ 1.65 ms (830 TFLOP/s), dK / dV 2.57 ms
-// (710 TFLOP/s) and 0.11 ms for the sums over the parts of the heads;  32 utterances of 600 .. 800 rows, 2 heads of 128: 55 and 71 us.  Bound like the forward
+// Measured (bf16, 16 heads of 128 sharing 4, capped scores, 5 documents of 1000 .. 8192 rows under a prefix mask): dQ 1.62 ms (845 TFLOP/s), dK / dV 2.51 ms
+// (730 TFLOP/s) and 0.11 ms for the sums over the parts of the heads;  32 utterances of 600 .. 800 rows, 2 heads of 128: 54 and 70 us.  Bound like the forward
 // (attention_packed_fwd.hip); the cap costs two transcendentals more per score in each kernel.
 #include "attention_packed_common.h"
 #include <type_traits>

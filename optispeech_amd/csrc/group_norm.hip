@@ -16,8 +16,8 @@
 // themselves (a launch of its own does it where a document has many).  Backward: per-channel partials -> per-document sums -> apply, the
 // sum of the documents' dw / db riding on the last launch.
 //
-// Measured: 37 k rows x 384 channels bf16, 8 groups, silu: forward 18.4 us (3.1 TB/s), backward 35.5 + 3.9 us (the silu and its slope, evaluated twice, take 11 of
-// them);  23 k rows x 256 channels f32, 32 groups, gelu: 17.2 and 30.7 + 3.9 us.  Twice through memory instead: 28 and 43 us, 25 and 45 us.
+// Measured: 37 k rows x 384 channels bf16, 8 groups, silu: forward 18.3 us (3.1 TB/s), backward 35.2 + 3.9 us (the silu and its slope, evaluated twice, take 11 of
+// them);  23 k rows x 256 channels f32, 32 groups, gelu: 17.4 and 30.9 + 4.0 us.  Twice through memory instead: 28 and 43 us, 25 and 45 us.
 #include "packed_common.h"
 
 namespace {
