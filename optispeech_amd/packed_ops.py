@@ -252,6 +252,10 @@ def _grad_target(p):
     return (p.grad, 1) if p.grad.is_contiguous() else (torch.empty_like(p), 0)
 
 
+def _version(p):
+    return None if p is None or p.is_inference() else p._version
+
+
 class GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, anchor, wc, bc, params, groups, rows, eps, act):
@@ -260,6 +264,7 @@ class GroupNormFn(torch.autograd.Function):
         x, y, stats = _normalise(x, w, b, groups, rows, eps, act)
         ctx.save_for_backward(x, stats, wc, bc)
         ctx.params, ctx.cfg = params, (groups, rows, act)
+        ctx.versions = [_version(p) for p in params]
         return y
 
     @staticmethod
@@ -267,6 +272,8 @@ class GroupNormFn(torch.autograd.Function):
         _first_order()
         x, stats, wc, bc = ctx.saved_tensors
         (w, b), (groups, rows, act) = ctx.params, ctx.cfg
+        if ctx.versions != [_version(w), _version(b)]:             # as autograd does for the tensors it keeps itself
+            raise OspError("a weight or bias of group_norm has been modified by an inplace operation between its forward and backward")
         M, C = x.shape
         dy = _matrix(dy, "dy")
         dx = torch.empty((M, C), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None

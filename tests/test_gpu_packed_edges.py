@@ -403,3 +403,25 @@ def test_new_tokens_for_many_documents(monkeypatch):
                            torch.bfloat16)
         close((o[b:b + 1],), want[:1], tol[:1])
     assert float(o[B:].abs().max()) == 0.0
+
+
+@gpu
+def test_group_norm_parameters_changed_before_the_backward_are_refused():
+    """the gradients would be those of other weights: in-place steps in between raise, frozen weights and those of inference mode are used as they are"""
+    from optispeech_amd import packed_ops as P
+    rows = P.PackedRows.from_offsets(offsets([30, 11]), 41)
+    x, g = randn(41, 32, seed=1).requires_grad_(), randn(41, 32, seed=2)
+    for which in (0, 1):
+        p = [torch.nn.Parameter(randn(32, seed=3)), torch.nn.Parameter(randn(32, seed=4))]
+        y = P.group_norm(x, *p, 4, rows, act="silu")
+        with torch.no_grad():
+            p[which] += 0.1
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward(g)
+        assert p[0].grad is None and p[1].grad is None
+        P.group_norm(x, *p, 4, rows, act="silu").backward(g)
+    with torch.inference_mode():
+        w, b = randn(32, seed=3), randn(32, seed=4)
+    (a,) = torch.autograd.grad(P.group_norm(x, w, b, 4, rows, act="silu"), (x,), g)
+    (c,) = torch.autograd.grad(P.group_norm(x, w.clone(), b.clone(), 4, rows, act="silu"), (x,), g)
+    assert torch.equal(a, c)
